@@ -1,8 +1,13 @@
-"""B200-native Walsh-Hadamard transform and fused W . H(X).
+"""B200-native Walsh-Hadamard transform, fused W . H(X), and the operators of a model around them.
 
 The directory name starts with a digit, so import it with
 ``importlib.import_module("6s894_project_2025_b200")``.
 """
+from .heads import (  # noqa: F401
+    norm_rotary_qk,
+    norm_rotary_qk_backward,
+    rotary_qk,
+)
 from .ops import (  # noqa: F401
     HostPipeline,
     device_status,
@@ -28,6 +33,9 @@ __all__ = [
     "fused_ht_gemm",
     "fused_ht_gemv",
     "fused_gemm_workspace_bytes",
+    "rotary_qk",
+    "norm_rotary_qk",
+    "norm_rotary_qk_backward",
     "device_status",
     "token_range",
     "shard_tokens",

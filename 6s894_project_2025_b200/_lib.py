@@ -15,6 +15,7 @@ LIB_PATH = _HERE / "libb200ht.so"
 F16, BF16, F32 = 0, 1, 2
 OUT_MN, OUT_NM = 0, 1
 STATIC_SCRATCH_BYTES = 32 << 20
+ROT_INTERLEAVED, ROT_HADAMARD, ROT_INVERSE, ROT_POS64, ROT_WEIGHT_F32 = 1, 2, 4, 8, 16
 
 # every symbol include/b200ht.h declares
 EXPORTS = (
@@ -31,6 +32,9 @@ EXPORTS = (
     "b200ht_fused_gemv",
     "b200ht_fused_gemv_max_batch",
     "b200ht_fused_gemv_peers",
+    "b200ht_rotary_qk",
+    "b200ht_norm_rotary_qk_backward",
+    "b200ht_norm_rotary_qk_backward_workspace_bytes",
     "b200ht_ipc_export",
     "b200ht_ipc_open",
     "b200ht_ipc_close",
@@ -72,6 +76,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.b200ht_fused_gemv_peers.restype = i
     lib.b200ht_fused_gemv_peers.argtypes = [vp, vp, vp, i, i, i, i, i, f, i, i, i, ctypes.POINTER(vp), vp, vp,
                                             ctypes.c_uint, vp]
+    ll = ctypes.c_longlong
+    lib.b200ht_rotary_qk.restype = i
+    lib.b200ht_rotary_qk.argtypes = [vp, vp, vp, vp, vp, vp, f, i, i, i, i, ctypes.POINTER(ll), i, vp, ll, ll, i,
+                                     ctypes.c_char_p, vp, i, i, vp]
+    lib.b200ht_norm_rotary_qk_backward_workspace_bytes.restype = ctypes.c_size_t
+    lib.b200ht_norm_rotary_qk_backward_workspace_bytes.argtypes = [i]
+    lib.b200ht_norm_rotary_qk_backward.restype = i
+    lib.b200ht_norm_rotary_qk_backward.argtypes = [vp, vp, vp, vp, vp, vp, f, vp, vp, vp, vp, i, i, i, i,
+                                                   ctypes.POINTER(ll), i, vp, ll, ll, i, ctypes.c_char_p, vp, i, i, vp,
+                                                   ctypes.c_size_t, vp]
     lib.b200ht_ipc_export.restype = i
     lib.b200ht_ipc_export.argtypes = [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_ulonglong)]
     lib.b200ht_ipc_open.restype = i

@@ -231,6 +231,52 @@ int b200ht_ipc_open(const void *handle64, void **base);
 int b200ht_ipc_close(void *base);
 
 /*
+ * Position rotation of queries and keys, optionally behind an RMS norm of every head, optionally followed by the
+ * Hadamard rotation of the head dimension, in one pass.  No counterpart in the reference.
+ *   q, k          `tokens` x heads x head_dim, the last dimension contiguous; q_out, k_out: the same (q_out == q with
+ *                 the same strides rotates in place; other overlaps are the caller's error)
+ *   strides       8 numbers in HOST memory, in elements: token and head stride of q, of k, of q_out, of k_out
+ *   q_weight, k_weight   head_dim values each: y = x * rsqrt(mean(x^2) + eps) * weight comes first.  Both NULL: no norm
+ *   positions     one integer per token and axis: element axis * pos_axis_stride + token * pos_token_stride, 32 bits or
+ *                 (B200HT_ROT_POS64) 64 bits
+ *   axis_of_pair  `pairs` bytes in HOST memory, the axis (< n_axes <= 4) whose position turns each pair; NULL with one axis
+ *   inv_freq      `pairs` floats, radians per unit of position; dimensions from 2 * pairs on are not rotated
+ *   flags         B200HT_ROT_INTERLEAVED: pair i is dimensions (2i, 2i+1), else (i, i + pairs)
+ *                 B200HT_ROT_HADAMARD: . H / sqrt(head_dim) after the rotation (head_dim a power of two)
+ *                 B200HT_ROT_INVERSE: the transposed steps in reverse order, which is the gradient (no norm)
+ *                 B200HT_ROT_WEIGHT_F32: the weights are floats, not `dtype`
+ * head_dim is even, 2 .. 256; dtype F16 | BF16 | F32.  fp32 arithmetic (fp64 for the angle), one rounding on the store.
+ * Pointers need the alignment of their element type; 16-byte aligned rows of a multiple of 16 elements run fastest.
+ */
+#define B200HT_ROT_INTERLEAVED 1
+#define B200HT_ROT_HADAMARD    2
+#define B200HT_ROT_INVERSE     4
+#define B200HT_ROT_POS64       8
+#define B200HT_ROT_WEIGHT_F32 16
+int b200ht_rotary_qk(const void *q, const void *k, void *q_out, void *k_out, const void *q_weight,
+                     const void *k_weight, float eps, int tokens, int q_heads, int k_heads, int head_dim,
+                     const long long *strides, int dtype, const void *positions, long long pos_axis_stride,
+                     long long pos_token_stride, int n_axes, const unsigned char *axis_of_pair, const float *inv_freq,
+                     int pairs, int flags, void *stream);
+
+/*
+ * Gradient of b200ht_rotary_qk with a norm.  dq_out, dk_out are the gradients of its results, q and k its inputs;
+ * dq, dk receive the gradients of the inputs, dq_weight, dk_weight (head_dim values of the weights' type) those of the
+ * weights, summed over tokens and heads in fp32 in an order that does not change from call to call.
+ *   strides    12 numbers in HOST memory: token and head stride of dq_out, dk_out, q, k, dq, dk
+ *   workspace  b200ht_norm_rotary_qk_backward_workspace_bytes(head_dim) bytes, 16-byte aligned
+ * With tokens == 0 the weights' gradients are set to zero.  Everything else as b200ht_rotary_qk.
+ */
+size_t b200ht_norm_rotary_qk_backward_workspace_bytes(int head_dim);
+int b200ht_norm_rotary_qk_backward(const void *dq_out, const void *dk_out, const void *q, const void *k,
+                                   const void *q_weight, const void *k_weight, float eps, void *dq, void *dk,
+                                   void *dq_weight, void *dk_weight, int tokens, int q_heads, int k_heads, int head_dim,
+                                   const long long *strides, int dtype, const void *positions, long long pos_axis_stride,
+                                   long long pos_token_stride, int n_axes, const unsigned char *axis_of_pair,
+                                   const float *inv_freq, int pairs, int flags, void *workspace, size_t workspace_bytes,
+                                   void *stream);
+
+/*
  * Number of kernels this library has launched in the calling process so far (all entry points, all streams).
  * A benchmark reads it before and after a timed region to report its launch count.  No counterpart in the reference.
  */
