@@ -210,6 +210,398 @@ norm_rotary_any_grad_kernel(const __grid_constant__ RotArgs a, int q_blocks)
     }
 }
 
+// ---------------------------------------------------------------------------
+// The fast form, for rows of 16-byte vectors: head_dim a multiple of 16, every row on a 16-byte boundary, and pairs that
+// are neighbours, or halves of the whole head, or lie in its first half eight by eight.
+//
+// A group of LANES lanes (the power of two from head_dim / 16 on) holds a row in registers: lane j has dimensions
+// 8j .. 8j + 7 and head_dim / 2 + the same, so both members of a split pair, and the top bit of the index for H, meet in
+// one lane; H needs shuffles for log2(head_dim) - 4 bits only.  A block of 256 threads takes `tb` tokens: cos and sin of
+// their pairs are computed once into shared memory and serve all heads, each group walks over heads of one token with
+// the next row's loads in flight.  Bound: HBM; with H the instruction rate is next (about 200 issued instructions per
+// 512 values and warp), hence the packed fp32 instructions.
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;\n"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+          "l"(reinterpret_cast<unsigned long long &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, make_float2(-1.f, -1.f), a); }
+
+// The two vectors of a lane as they lie in memory, and as fp32: v[s][i] = dimensions 2i, 2i + 1 of vector s.
+template <int DT>
+struct RowRaw {
+    uint4 v[2][DT == B200HT_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ void row_load(RowRaw<DT> &r, const void *x, long long at, int half)
+{
+    constexpr int size = DT == B200HT_F32 ? 4 : 2;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const uint4 *p = (const uint4 *)((const unsigned char *)x + (at + s * half) * size);
+#pragma unroll
+        for (int i = 0; i < size / 2; ++i) r.v[s][i] = p[i];
+    }
+}
+template <int DT>
+__device__ __forceinline__ void row_unpack(const RowRaw<DT> &r, float2 (&v)[2][4])
+{
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if constexpr (DT == B200HT_F32) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[s][2 * i] = make_float2(__uint_as_float(r.v[s][i].x), __uint_as_float(r.v[s][i].y));
+                v[s][2 * i + 1] = make_float2(__uint_as_float(r.v[s][i].z), __uint_as_float(r.v[s][i].w));
+            }
+        } else {
+            v[s][0] = unpack2<DT>(r.v[s][0].x);
+            v[s][1] = unpack2<DT>(r.v[s][0].y);
+            v[s][2] = unpack2<DT>(r.v[s][0].z);
+            v[s][3] = unpack2<DT>(r.v[s][0].w);
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void row_store(void *y, long long at, int half, const float2 (&v)[2][4])
+{
+    constexpr int size = DT == B200HT_F32 ? 4 : 2;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        uint4 *p = (uint4 *)((unsigned char *)y + (at + s * half) * size);
+        if constexpr (DT == B200HT_F32) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                p[i] = make_uint4(__float_as_uint(v[s][2 * i].x), __float_as_uint(v[s][2 * i].y),
+                                  __float_as_uint(v[s][2 * i + 1].x), __float_as_uint(v[s][2 * i + 1].y));
+        } else {
+            p[0] = make_uint4(pack2<DT>(v[s][0].x, v[s][0].y), pack2<DT>(v[s][1].x, v[s][1].y),
+                              pack2<DT>(v[s][2].x, v[s][2].y), pack2<DT>(v[s][3].x, v[s][3].y));
+        }
+    }
+}
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v)
+{
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// y = y . H / sqrt(D); `lanes` = D / 16 lanes hold the row, `c` = 1 / sqrt(D).
+template <int LANES>
+__device__ __forceinline__ void row_hadamard(float2 (&v)[2][4], int j, int lanes, float c)
+{
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[s][i] = make_float2(v[s][i].x + v[s][i].y, v[s][i].x - v[s][i].y);
+#pragma unroll
+        for (int m = 1; m < 4; m <<= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!(i & m)) {
+                    const float2 a = v[s][i], b = v[s][i | m];
+                    v[s][i] = add2(a, b);
+                    v[s][i | m] = sub2(a, b);
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = v[0][i], b = v[1][i];
+        v[0][i] = add2(a, b);
+        v[1][i] = sub2(a, b);
+    }
+#pragma unroll
+    for (int m = 1; m < LANES; m <<= 1) {
+        if (m < lanes) {
+            const float sg = (j & m) ? -1.f : 1.f;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 o = make_float2(__shfl_xor_sync(0xffffffffu, v[s][i].x, m),
+                                                 __shfl_xor_sync(0xffffffffu, v[s][i].y, m));
+                    v[s][i] = fma2(v[s][i], make_float2(sg, sg), o);
+                }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[s][i] = mul2(v[s][i], make_float2(c, c));
+}
+
+// How the pairs lie in a lane's registers.
+enum { kPairsNeighbour, kPairsHalves, kPairsInFirstHalf };
+
+// cos and sin of the lane's pairs: c[i], s[i] are those of dimensions 2i, 2i + 1 of vector 0 (and of vector 1: split over
+// the whole head, both vectors have the same pairs); for neighbours c[0..1] are vector 0's four pairs, c[2..3] vector 1's.
+struct RowTurn {
+    float2 c[4], s[4];
+};
+
+__device__ __forceinline__ void row_turn(RowTurn &t, const float2 *tab, int mode, int j, int D, int pairs)
+{
+    if (mode == kPairsNeighbour) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 cs = tab[(i >> 2) * (D / 4) + 4 * j + (i & 3)];
+            (i & 1 ? t.c[i >> 1].y : t.c[i >> 1].x) = cs.x;
+            (i & 1 ? t.s[i >> 1].y : t.s[i >> 1].x) = cs.y;
+        }
+        return;
+    }
+    // split pairs in the first half: the second member's lane has them `pairs` dimensions on, with sin's sign turned
+    const int e = 8 * j;
+    const bool second = mode == kPairsInFirstHalf && e >= pairs;
+    const bool none = mode == kPairsInFirstHalf && e >= 2 * pairs;
+    const int first = second ? e - pairs : e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 cs = none ? make_float2(1.f, 0.f) : tab[first + i];
+        (i & 1 ? t.c[i >> 1].y : t.c[i >> 1].x) = cs.x;
+        (i & 1 ? t.s[i >> 1].y : t.s[i >> 1].x) = mode == kPairsInFirstHalf && !second ? -cs.y : cs.y;
+    }
+}
+
+__device__ __forceinline__ void row_rotate(float2 (&v)[2][4], const RowTurn &t, int mode, int partner)
+{
+    if (mode == kPairsHalves) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = v[0][i], b = v[1][i];
+            const float2 as = mul2(a, t.s[i]), bs = mul2(b, make_float2(-t.s[i].x, -t.s[i].y));
+            v[0][i] = fma2(a, t.c[i], bs);
+            v[1][i] = fma2(b, t.c[i], as);
+        }
+    } else if (mode == kPairsNeighbour) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float c = i & 1 ? t.c[2 * s + (i >> 1)].y : t.c[2 * s + (i >> 1)].x;
+                const float sn = i & 1 ? t.s[2 * s + (i >> 1)].y : t.s[2 * s + (i >> 1)].x;
+                const float a = v[s][i].x, b = v[s][i].y;
+                v[s][i] = make_float2(a * c - b * sn, b * c + a * sn);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 o = make_float2(__shfl_sync(0xffffffffu, v[0][i].x, partner), __shfl_sync(0xffffffffu, v[0][i].y, partner));
+            v[0][i] = fma2(o, t.s[i], mul2(v[0][i], t.c[i]));
+        }
+    }
+}
+
+// cos and sin of `tb` tokens' pairs, D / 2 entries a token; entries behind the pairs turn nothing.
+__device__ __forceinline__ void fill_turns(float2 *tab, const RotArgs &a, int token0, int tb)
+{
+    const int half = a.D / 2;
+    for (int i = threadIdx.x; i < tb * half; i += kRowThreads) {
+        const int tk = i / half, pair = i - tk * half, token = token0 + tk;
+        float2 cs = make_float2(1.f, 0.f);
+        if (pair < a.pairs && token < a.tokens) {
+            cs = rot_cos_sin(a, token, pair);
+            if (a.inverse) cs.y = -cs.y;
+        }
+        tab[i] = cs;
+    }
+}
+
+// Lane of a warp that holds the other member of this lane's split pairs in the first half (pairs a multiple of 8).
+__device__ __forceinline__ int row_partner(int mode, int j, int pairs)
+{
+    const int lane = threadIdx.x & 31;
+    if (mode != kPairsInFirstHalf || 8 * j >= 2 * pairs) return lane;
+    return 8 * j < pairs ? lane + pairs / 8 : lane - pairs / 8;
+}
+
+template <int DT, bool NORM, bool HAD, int LANES>
+__global__ void __launch_bounds__(kRowThreads)
+rotary_row_kernel(const __grid_constant__ RotArgs a, int tb, int mode)
+{
+    extern __shared__ float2 tab[];                  // [tb][D / 2], then the weights: [2][D] floats
+    constexpr int GROUPS = kRowThreads / LANES;
+    const int D = a.D, half = D / 2, lanes = D / 16;
+    float *wts = (float *)(tab + tb * half);
+    const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
+    const int per = GROUPS / tb, tk = group / per;   // groups of one token
+    const int token0 = blockIdx.x * tb, token = token0 + tk;
+    const int heads = a.t[0].heads + a.t[1].heads;
+    const int steps = (heads + per - 1) / per;
+    const bool mine = token < a.tokens && j < lanes;
+    int h = group - tk * per;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    auto row = [&](int head, bool out) {
+        const int which = head < a.t[0].heads ? 0 : 1;
+        const int hh = which ? head - a.t[0].heads : head;
+        const RotTensor &t = a.t[which];
+        return out ? token * t.y_tok + hh * t.y_head + 8 * j : token * t.x_tok + hh * t.x_head + 8 * j;
+    };
+    RowRaw<DT> next = {};
+    if (mine && h < heads) row_load<DT>(next, h < a.t[0].heads ? a.t[0].x : a.t[1].x, row(h, false), half);
+    fill_turns(tab, a, token0, tb);
+    if constexpr (NORM)
+        for (int i = threadIdx.x; i < 2 * D; i += kRowThreads) {
+            const void *w = i < D ? a.t[0].w : a.t[1].w;
+            wts[i] = w ? rot_weight<DT>(a, w, i < D ? i : i - D) : 0.f;
+        }
+    __syncthreads();
+    RowTurn turn;
+    const int jj = j < lanes ? j : 0;
+    row_turn(turn, tab + tk * half, mode, jj, D, a.pairs);
+    const int partner = row_partner(mode, j, a.pairs);
+    const float hc = HAD ? rsqrtf((float)D) : 1.f;
+
+    for (int step = 0; step < steps; ++step, h += per) {
+        const RowRaw<DT> cur = next;
+        if (mine && h + per < heads)
+            row_load<DT>(next, h + per < a.t[0].heads ? a.t[0].x : a.t[1].x, row(h + per, false), half);
+        float2 v[2][4];
+        row_unpack<DT>(cur, v);
+        if constexpr (NORM) {
+            float2 q = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q = fma2(v[s][i], v[s][i], q);
+            const float sum = row_sum<LANES>(j < lanes ? q.x + q.y : 0.f);
+            const float r = rsqrtf(sum / (float)D + a.eps);
+            const float *w = wts + (h < a.t[0].heads ? 0 : D);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[s][i] = mul2(mul2(v[s][i], make_float2(r, r)), *(const float2 *)(w + s * half + 8 * jj + 2 * i));
+        }
+        if (HAD && !NORM && a.inverse) row_hadamard<LANES>(v, j, lanes, hc);
+        row_rotate(v, turn, mode, partner);
+        if (HAD && (NORM || !a.inverse)) row_hadamard<LANES>(v, j, lanes, hc);
+        if (mine && h < heads) row_store<DT>(h < a.t[0].heads ? a.t[0].y : a.t[1].y, row(h, true), half, v);
+    }
+}
+
+// Gradient of norm and rotation, the same layout.  The first `q_blocks` blocks serve the queries, the others the keys;
+// a block walks over tiles of tb tokens and keeps its share of the weights' gradient in registers until the end.
+template <int DT, bool HAD, int LANES>
+__global__ void __launch_bounds__(kRowThreads)
+norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int tb, int mode, int q_blocks)
+{
+    extern __shared__ float2 tab[];                  // [tb][D / 2], at the end [groups][D] floats
+    __shared__ float wts[kMaxHeadDim];
+    constexpr int GROUPS = kRowThreads / LANES;
+    const int D = a.D, half = D / 2, lanes = D / 16;
+    const int which = (int)blockIdx.x < q_blocks ? 0 : 1;
+    const int block = which ? (int)blockIdx.x - q_blocks : (int)blockIdx.x;
+    const int blocks = which ? (int)gridDim.x - q_blocks : q_blocks;
+    const RotTensor &t = a.t[which];
+    const int group = threadIdx.x / LANES, j = threadIdx.x % LANES, jj = j < lanes ? j : 0;
+    const int per = GROUPS / tb, tk = group / per, h0 = group - tk * per;
+    const int steps = (t.heads + per - 1) / per;
+    const int partner = row_partner(mode, j, a.pairs);
+    const float hc = HAD ? rsqrtf((float)D) : 1.f, inv_d = 1.f / (float)D;
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int i = threadIdx.x; i < D; i += kRowThreads) wts[i] = rot_weight<DT>(a, t.w, i);
+
+    float2 dw[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dw[s][i] = make_float2(0.f, 0.f);
+
+    for (long long token0 = (long long)block * tb; token0 < a.tokens; token0 += (long long)blocks * tb) {
+        const int token = (int)token0 + tk;
+        const bool mine = token < a.tokens && j < lanes;
+        RowRaw<DT> nx = {}, ng = {};
+        if (mine && h0 < t.heads) {
+            row_load<DT>(nx, t.x, token * t.x_tok + h0 * t.x_head + 8 * j, half);
+            row_load<DT>(ng, t.g, token * t.g_tok + h0 * t.g_head + 8 * j, half);
+        }
+        __syncthreads();
+        fill_turns(tab, a, (int)token0, tb);   // a.inverse is set: the gradient turns back
+        __syncthreads();
+        RowTurn turn;
+        row_turn(turn, tab + tk * half, mode, jj, D, a.pairs);
+        int h = h0;
+        for (int step = 0; step < steps; ++step, h += per) {
+            float2 x[2][4], g[2][4];
+            row_unpack<DT>(nx, x);
+            row_unpack<DT>(ng, g);
+            const bool on = mine && h < t.heads;
+            if (mine && h + per < t.heads) {
+                row_load<DT>(nx, t.x, token * t.x_tok + (h + per) * t.x_head + 8 * j, half);
+                row_load<DT>(ng, t.g, token * t.g_tok + (h + per) * t.g_head + 8 * j, half);
+            }
+            if (HAD) row_hadamard<LANES>(g, j, lanes, hc);
+            row_rotate(g, turn, mode, partner);
+            float2 q = make_float2(0.f, 0.f), d = make_float2(0.f, 0.f);
+            float2 gw[2][4];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    q = fma2(x[s][i], x[s][i], q);
+                    gw[s][i] = mul2(g[s][i], *(const float2 *)(wts + s * half + 8 * jj + 2 * i));
+                    d = fma2(x[s][i], gw[s][i], d);
+                }
+            const float sum = row_sum<LANES>(j < lanes ? q.x + q.y : 0.f);
+            const float dot = row_sum<LANES>(j < lanes ? d.x + d.y : 0.f);
+            const float r = rsqrtf(sum * inv_d + a.eps);
+            // dx = r (gw - h mean(gw h)), h = x r
+            const float k = -r * r * dot * inv_d;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (on) dw[s][i] = fma2(g[s][i], mul2(x[s][i], make_float2(r, r)), dw[s][i]);
+                    gw[s][i] = mul2(fma2(x[s][i], make_float2(k, k), gw[s][i]), make_float2(r, r));
+                }
+            if (on) row_store<DT>(t.y, token * t.y_tok + h * t.y_head + 8 * j, half, gw);
+        }
+    }
+
+    __syncthreads();
+    float *rows = (float *)tab;
+    if (j < lanes)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(float2 *)(rows + group * D + s * half + 8 * j + 2 * i) = dw[s][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += kRowThreads) {
+        float sum = 0.f;
+        for (int w = 0; w < GROUPS; ++w) sum += rows[w * D + i];
+        a.partial[(long long)blockIdx.x * D + i] = sum;
+    }
+}
+
 // dw[i] = sum of the blocks' rows, in a fixed order: 8 warps take every eighth row of 32 columns, then the warps are
 // added in order.  blockIdx.y: queries or keys.
 template <int DT>
@@ -268,7 +660,9 @@ static GradBlocks grad_blocks(long long q_rows, long long k_rows, long long rows
     if (k_rows && b.k < 1) b.k = 1;
     return b;
 }
-constexpr int kGradBlocks = 148 * 8;   // blocks of a gradient launch at most (one more may come from rounding up)
+// Blocks of a gradient launch at most (one more may come from rounding up).  They do not go by the device's number of
+// SMs, so that the order of the sums goes by the sizes alone.
+constexpr int kGradBlocks = 148 * 8, kRowGradBlocks = 148 * 3;
 
 static int check_rot_common(const RotArgs &a, int dtype, int flags, const unsigned char *axis_of_pair, int n_axes)
 {
@@ -306,23 +700,101 @@ static int check_rot_pointers(const RotArgs &a, int dtype, int flags)
     return 0;
 }
 
+// The layout of the fast form, or -1 where a row does not fit it.
+static int row_mode(const RotArgs &a, int dtype, bool grad)
+{
+    if (a.D % 16) return -1;
+    const long long vec = dtype == B200HT_F32 ? 4 : 8;
+    for (const RotTensor &t : a.t) {
+        if (!t.heads) continue;
+        if (!aligned16(t.x) || !aligned16(t.y) || t.x_tok % vec || t.x_head % vec || t.y_tok % vec || t.y_head % vec) return -1;
+        if (grad && (!aligned16(t.g) || t.g_tok % vec || t.g_head % vec)) return -1;
+    }
+    if (a.interleaved) return kPairsNeighbour;
+    if (2 * a.pairs == a.D) return kPairsHalves;
+    return a.pairs % 8 == 0 && 4 * a.pairs <= a.D ? kPairsInFirstHalf : -1;
+}
+
+// Tokens of a block: as many as keep its groups busy (the last step of the walk over the heads may leave some idle)
+// with several rows a group, so that cos and sin and the start of the block are shared; one where there are few tokens
+// and all SMs can have a block of their own.
+static int row_tokens(int groups, int heads, int tokens)
+{
+    if (tokens <= 2 * sm_count()) return 1;
+    int best = 1;
+    double best_use = 0;
+    for (int tb = 1; tb <= groups && tb <= 16; tb *= 2) {
+        const int per = groups / tb, steps = (heads + per - 1) / per;
+        if (steps > 8 && best_use > 0) break;
+        const double use = (double)heads / (per * steps) * steps / (steps + 0.5);
+        if (use > best_use) { best_use = use; best = tb; }
+    }
+    return best;
+}
+
+template <int DT, bool NORM, int LANES>
+static int launch_rows(const RotArgs &a, bool had, int mode, cudaStream_t st)
+{
+    const int tb = row_tokens(kRowThreads / LANES, a.t[0].heads + a.t[1].heads, a.tokens);
+    const size_t smem = (size_t)tb * (a.D / 2) * sizeof(float2) + (NORM ? (size_t)2 * a.D * sizeof(float) : 0);
+    const dim3 grid((unsigned)((a.tokens + tb - 1) / tb)), block(kRowThreads);
+    return had ? launch_pdl(rotary_row_kernel<DT, NORM, true, LANES>, grid, block, smem, st, a, tb, mode)
+               : launch_pdl(rotary_row_kernel<DT, NORM, false, LANES>, grid, block, smem, st, a, tb, mode);
+}
+
+template <int DT, bool NORM>
+static int launch_forward(const RotArgs &a, bool had, int dtype, cudaStream_t st)
+{
+    const int mode = row_mode(a, dtype, false);
+    if (mode < 0) return launch_any<DT, NORM>(a, had, st);
+    if (a.D <= 64) return launch_rows<DT, NORM, 4>(a, had, mode, st);
+    if (a.D <= 128) return launch_rows<DT, NORM, 8>(a, had, mode, st);
+    return launch_rows<DT, NORM, 16>(a, had, mode, st);
+}
 template <int DT>
 static int launch_rotary(const RotArgs &a, bool norm, bool had, cudaStream_t st)
 {
-    return norm ? launch_any<DT, true>(a, had, st) : launch_any<DT, false>(a, had, st);
+    return norm ? launch_forward<DT, true>(a, had, DT, st) : launch_forward<DT, false>(a, had, DT, st);
+}
+
+template <int DT, int LANES>
+static int launch_row_grad(const RotArgs &a, bool had, int mode, GradBlocks *b, cudaStream_t st)
+{
+    constexpr int groups = kRowThreads / LANES;
+    const int tb = row_tokens(groups, a.t[0].heads > a.t[1].heads ? a.t[0].heads : a.t[1].heads, a.tokens);
+    const long long q_rows = (long long)a.tokens * a.t[0].heads, k_rows = (long long)a.tokens * a.t[1].heads;
+    *b = grad_blocks(q_rows, k_rows, groups, kRowGradBlocks);
+    if (b->q + b->k == 0) return 0;
+    const size_t table = (size_t)tb * (a.D / 2) * sizeof(float2), rows = (size_t)groups * a.D * sizeof(float);
+    const dim3 grid((unsigned)(b->q + b->k)), block(kRowThreads);
+    const size_t smem = table > rows ? table : rows;
+    return had ? launch_pdl(norm_rotary_row_grad_kernel<DT, true, LANES>, grid, block, smem, st, a, tb, mode, b->q)
+               : launch_pdl(norm_rotary_row_grad_kernel<DT, false, LANES>, grid, block, smem, st, a, tb, mode, b->q);
 }
 
 template <int DT>
-static int launch_norm_grad(const RotArgs &a, bool had, void *dwq, void *dwk, cudaStream_t st)
+static int launch_norm_grad(RotArgs &a, bool had, void *dwq, void *dwk, cudaStream_t st)
 {
     const long long q_rows = (long long)a.tokens * a.t[0].heads, k_rows = (long long)a.tokens * a.t[1].heads;
-    const GradBlocks b = grad_blocks(q_rows, k_rows, kAnyWarps, kGradBlocks);
-    if (b.q + b.k) {
-        const dim3 grid((unsigned)(b.q + b.k)), block(32 * kAnyWarps);
-        const int rc = had ? launch_pdl(norm_rotary_any_grad_kernel<DT, true>, grid, block, 0, st, a, b.q)
-                           : launch_pdl(norm_rotary_any_grad_kernel<DT, false>, grid, block, 0, st, a, b.q);
-        if (rc) return rc;
+    const int mode = row_mode(a, DT, true);
+    a.inverse = 1;
+    GradBlocks b{0, 0};
+    int rc = 0;
+    if (mode < 0) {
+        b = grad_blocks(q_rows, k_rows, kAnyWarps, kGradBlocks);
+        if (b.q + b.k) {
+            const dim3 grid((unsigned)(b.q + b.k)), block(32 * kAnyWarps);
+            rc = had ? launch_pdl(norm_rotary_any_grad_kernel<DT, true>, grid, block, 0, st, a, b.q)
+                     : launch_pdl(norm_rotary_any_grad_kernel<DT, false>, grid, block, 0, st, a, b.q);
+        }
+    } else if (a.D <= 64) {
+        rc = launch_row_grad<DT, 4>(a, had, mode, &b, st);
+    } else if (a.D <= 128) {
+        rc = launch_row_grad<DT, 8>(a, had, mode, &b, st);
+    } else {
+        rc = launch_row_grad<DT, 16>(a, had, mode, &b, st);
     }
+    if (rc) return rc;
     return launch_pdl(norm_weight_grad_kernel<DT>, dim3((unsigned)((a.D + 31) / 32), 2), dim3(256), 0, st, (const float *)a.partial,
                       b.q, b.k, a.D, dwq, dwk, a.w_f32);
 }
