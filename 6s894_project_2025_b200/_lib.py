@@ -78,13 +78,13 @@ def _declare(lib: ctypes.CDLL) -> None:
                                             ctypes.c_uint, vp]
     ll = ctypes.c_longlong
     lib.b200ht_rotary_qk.restype = i
-    lib.b200ht_rotary_qk.argtypes = [vp, vp, vp, vp, vp, vp, f, i, i, i, i, ctypes.POINTER(ll), i, vp, ll, ll, i,
+    lib.b200ht_rotary_qk.argtypes = [vp, vp, vp, vp, vp, vp, f, i, i, i, i, vp, i, vp, ll, ll, i,
                                      ctypes.c_char_p, vp, i, i, vp]
     lib.b200ht_norm_rotary_qk_backward_workspace_bytes.restype = ctypes.c_size_t
     lib.b200ht_norm_rotary_qk_backward_workspace_bytes.argtypes = [i]
     lib.b200ht_norm_rotary_qk_backward.restype = i
     lib.b200ht_norm_rotary_qk_backward.argtypes = [vp, vp, vp, vp, vp, vp, f, vp, vp, vp, vp, i, i, i, i,
-                                                   ctypes.POINTER(ll), i, vp, ll, ll, i, ctypes.c_char_p, vp, i, i, vp,
+                                                   vp, i, vp, ll, ll, i, ctypes.c_char_p, vp, i, i, vp,
                                                    ctypes.c_size_t, vp]
     lib.b200ht_ipc_export.restype = i
     lib.b200ht_ipc_export.argtypes = [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_ulonglong)]

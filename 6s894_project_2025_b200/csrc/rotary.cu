@@ -38,7 +38,7 @@ struct RotArgs {
     const float *inv_freq;
     float *partial;     // gradient of the weights: one row of D floats per block
     int tokens, D, pairs;
-    int pos64, w_f32, interleaved, inverse;
+    int n_axes, pos64, w_f32, interleaved, inverse;
     float eps;
     unsigned char axis[kMaxHeadDim / 2];
 };
@@ -47,7 +47,7 @@ struct RotArgs {
 // 32-bit position and a frequency is good to 2^-21 turns at worst; the rest is good to a few 2^-24.
 __device__ __forceinline__ float2 rot_cos_sin(const RotArgs &a, int token, int pair)
 {
-    const long long at = (long long)a.axis[pair] * a.pos_axis + (long long)token * a.pos_tok;
+    const long long at = (a.n_axes > 1 ? a.axis[pair] * a.pos_axis : 0) + token * a.pos_tok;
     const double p = a.pos64 ? (double)((const long long *)a.pos)[at] : (double)((const int *)a.pos)[at];
     double u = p * ((double)a.inv_freq[pair] * 0.15915494309189533577);
     u -= rint(u);
@@ -248,23 +248,28 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
           "l"(reinterpret_cast<unsigned long long &>(c)));
     return d;
 }
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, make_float2(-1.f, -1.f), a); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b)
+{
+    float2 d;
+    asm("sub.rn.f32x2 %0, %1, %2;\n"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return d;
+}
 
 // The two vectors of a lane as they lie in memory, and as fp32: v[s][i] = dimensions 2i, 2i + 1 of vector s.
 template <int DT>
 struct RowRaw {
     uint4 v[2][DT == B200HT_F32 ? 2 : 1];
 };
+// `p` is the lane's first vector; the second lies `half` bytes on.
 template <int DT>
-__device__ __forceinline__ void row_load(RowRaw<DT> &r, const void *x, long long at, int half)
+__device__ __forceinline__ void row_load(RowRaw<DT> &r, const unsigned char *p, int half)
 {
-    constexpr int size = DT == B200HT_F32 ? 4 : 2;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const uint4 *p = (const uint4 *)((const unsigned char *)x + (at + s * half) * size);
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int i = 0; i < size / 2; ++i) r.v[s][i] = p[i];
-    }
+        for (int i = 0; i < (DT == B200HT_F32 ? 2 : 1); ++i) r.v[s][i] = ((const uint4 *)(p + s * half))[i];
 }
 template <int DT>
 __device__ __forceinline__ void row_unpack(const RowRaw<DT> &r, float2 (&v)[2][4])
@@ -286,12 +291,11 @@ __device__ __forceinline__ void row_unpack(const RowRaw<DT> &r, float2 (&v)[2][4
     }
 }
 template <int DT>
-__device__ __forceinline__ void row_store(void *y, long long at, int half, const float2 (&v)[2][4])
+__device__ __forceinline__ void row_store(unsigned char *q, int half, const float2 (&v)[2][4])
 {
-    constexpr int size = DT == B200HT_F32 ? 4 : 2;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        uint4 *p = (uint4 *)((unsigned char *)y + (at + s * half) * size);
+        uint4 *p = (uint4 *)(q + s * half);
         if constexpr (DT == B200HT_F32) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -303,6 +307,19 @@ __device__ __forceinline__ void row_store(void *y, long long at, int half, const
         }
     }
 }
+// Weights as the lanes read them: four dimensions (16 bytes) of each lane side by side.
+template <int DT>
+__device__ __forceinline__ void fill_weights(float *wts, const RotArgs &a, const void *w, int D, int lanes)
+{
+    for (int i = threadIdx.x; i < D; i += kRowThreads) {
+        const int s = i / (D / 2), e = i - s * (D / 2);   // vector, dimension within the half
+        wts[((2 * s + ((e >> 2) & 1)) * lanes + (e >> 3)) * 4 + (e & 3)] = rot_weight<DT>(a, w, i);
+    }
+}
+__device__ __forceinline__ float4 row_weights(const float *wts, int s, int i, int j, int lanes)   // dimensions 4i .. 4i + 3
+{
+    return *(const float4 *)(wts + ((2 * s + i) * lanes + j) * 4);
+}
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v)
 {
@@ -311,9 +328,9 @@ __device__ __forceinline__ float row_sum(float v)
     return v;
 }
 
-// y = y . H / sqrt(D); `lanes` = D / 16 lanes hold the row, `c` = 1 / sqrt(D).
+// y = y . H; `lanes` = D / 16 lanes hold the row.
 template <int LANES>
-__device__ __forceinline__ void row_hadamard(float2 (&v)[2][4], int j, int lanes, float c)
+__device__ __forceinline__ void row_hadamard(float2 (&v)[2][4], int j, int lanes)
 {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -349,6 +366,9 @@ __device__ __forceinline__ void row_hadamard(float2 (&v)[2][4], int j, int lanes
                 }
         }
     }
+}
+__device__ __forceinline__ void row_scale(float2 (&v)[2][4], float c)
+{
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -394,9 +414,8 @@ __device__ __forceinline__ void row_rotate(float2 (&v)[2][4], const RowTurn &t, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 a = v[0][i], b = v[1][i];
-            const float2 as = mul2(a, t.s[i]), bs = mul2(b, make_float2(-t.s[i].x, -t.s[i].y));
-            v[0][i] = fma2(a, t.c[i], bs);
-            v[1][i] = fma2(b, t.c[i], as);
+            v[0][i] = sub2(mul2(a, t.c[i]), mul2(b, t.s[i]));
+            v[1][i] = fma2(b, t.c[i], mul2(a, t.s[i]));
         }
     } else if (mode == kPairsNeighbour) {
 #pragma unroll
@@ -417,18 +436,31 @@ __device__ __forceinline__ void row_rotate(float2 (&v)[2][4], const RowTurn &t, 
     }
 }
 
-// cos and sin of `tb` tokens' pairs, D / 2 entries a token; entries behind the pairs turn nothing.
-__device__ __forceinline__ void fill_turns(float2 *tab, const RotArgs &a, int token0, int tb)
+// cos and sin of `tb` tokens' pairs, D / 2 entries a token; entries behind the pairs turn nothing
+// (SPLIT: a token's D / 2 cosines, then its sines).  By THREADS threads, a block or a warp.
+template <int THREADS, bool SPLIT = false>
+__device__ __forceinline__ void fill_turns(float2 *tab, const RotArgs &a, long long token0, int tb)
 {
     const int half = a.D / 2;
-    for (int i = threadIdx.x; i < tb * half; i += kRowThreads) {
-        const int tk = i / half, pair = i - tk * half, token = token0 + tk;
+    auto entry = [&](int tk, int pair) {
         float2 cs = make_float2(1.f, 0.f);
-        if (pair < a.pairs && token < a.tokens) {
-            cs = rot_cos_sin(a, token, pair);
+        if (pair < a.pairs && token0 + tk < a.tokens) {
+            cs = rot_cos_sin(a, (int)token0 + tk, pair);
             if (a.inverse) cs.y = -cs.y;
         }
-        tab[i] = cs;
+        if (SPLIT) {
+            float *at = (float *)(tab + tk * half) + pair;
+            at[0] = cs.x;
+            at[half] = cs.y;
+        } else {
+            tab[tk * half + pair] = cs;
+        }
+    };
+    if (THREADS == 32) {
+        for (int tk = 0; tk < tb; ++tk)
+            for (int pair = threadIdx.x % 32; pair < half; pair += 32) entry(tk, pair);
+    } else {
+        for (int i = threadIdx.x % THREADS; i < tb * half; i += THREADS) entry(i / half, i % half);
     }
 }
 
@@ -441,94 +473,159 @@ __device__ __forceinline__ int row_partner(int mode, int j, int pairs)
 }
 
 template <int DT, bool NORM, bool HAD, int LANES>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, DT == B200HT_F32 ? 2 : 4)
 rotary_row_kernel(const __grid_constant__ RotArgs a, int tb, int mode)
 {
     extern __shared__ float2 tab[];                  // [tb][D / 2], then the weights: [2][D] floats
-    constexpr int GROUPS = kRowThreads / LANES;
+    constexpr int GROUPS = kRowThreads / LANES, SIZE = DT == B200HT_F32 ? 4 : 2;
     const int D = a.D, half = D / 2, lanes = D / 16;
     float *wts = (float *)(tab + tb * half);
     const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
     const int per = GROUPS / tb, tk = group / per;   // groups of one token
     const int token0 = blockIdx.x * tb, token = token0 + tk;
-    const int heads = a.t[0].heads + a.t[1].heads;
-    const int steps = (heads + per - 1) / per;
+    // the queries' heads come first, then the keys': each group has every per-th head
+    const int q_steps = (a.t[0].heads + per - 1) / per, steps = q_steps + (a.t[1].heads + per - 1) / per;
     const bool mine = token < a.tokens && j < lanes;
-    int h = group - tk * per;
+    const int h0 = group - tk * per;
     pdl_launch_dependents();
     pdl_wait();
 
-    auto row = [&](int head, bool out) {
-        const int which = head < a.t[0].heads ? 0 : 1;
-        const int hh = which ? head - a.t[0].heads : head;
-        const RotTensor &t = a.t[which];
-        return out ? token * t.y_tok + hh * t.y_head + 8 * j : token * t.x_tok + hh * t.x_head + 8 * j;
+    const unsigned char *in;
+    unsigned char *out;
+    long long in_step, out_step;
+    int left;                                        // heads of this tensor from the current one on
+    auto start = [&](const RotTensor &t) {
+        in = (const unsigned char *)t.x + (token * t.x_tok + h0 * t.x_head + 8 * j) * SIZE;
+        in_step = per * t.x_head * SIZE;
+        left = mine ? t.heads - h0 : 0;
+    };
+    auto start_out = [&](const RotTensor &t) {
+        out = (unsigned char *)t.y + (token * t.y_tok + h0 * t.y_head + 8 * j) * SIZE;
+        out_step = per * t.y_head * SIZE;
     };
     RowRaw<DT> next = {};
-    if (mine && h < heads) row_load<DT>(next, h < a.t[0].heads ? a.t[0].x : a.t[1].x, row(h, false), half);
-    fill_turns(tab, a, token0, tb);
-    if constexpr (NORM)
-        for (int i = threadIdx.x; i < 2 * D; i += kRowThreads) {
-            const void *w = i < D ? a.t[0].w : a.t[1].w;
-            wts[i] = w ? rot_weight<DT>(a, w, i < D ? i : i - D) : 0.f;
-        }
+    start(q_steps ? a.t[0] : a.t[1]);
+    start_out(q_steps ? a.t[0] : a.t[1]);
+    if (left > 0) row_load<DT>(next, in, half * SIZE);
+    fill_turns<kRowThreads>(tab, a, token0, tb);
+    if constexpr (NORM) {
+        if (a.t[0].heads) fill_weights<DT>(wts, a, a.t[0].w, D, lanes);
+        if (a.t[1].heads) fill_weights<DT>(wts + D, a, a.t[1].w, D, lanes);
+    }
     __syncthreads();
     RowTurn turn;
     const int jj = j < lanes ? j : 0;
     row_turn(turn, tab + tk * half, mode, jj, D, a.pairs);
     const int partner = row_partner(mode, j, a.pairs);
-    const float hc = HAD ? rsqrtf((float)D) : 1.f;
+    const float hc = HAD ? rsqrtf((float)D) : 1.f, inv_d = 1.f / (float)D;
 
-    for (int step = 0; step < steps; ++step, h += per) {
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
         const RowRaw<DT> cur = next;
-        if (mine && h + per < heads)
-            row_load<DT>(next, h + per < a.t[0].heads ? a.t[0].x : a.t[1].x, row(h + per, false), half);
+        const bool on = left > 0;
+        if (step + 1 == q_steps) {
+            if (step + 1 < steps) start(a.t[1]);
+        } else {
+            in += in_step;
+            left -= per;
+        }
+        if (step + 1 < steps && left > 0) row_load<DT>(next, in, half * SIZE);
         float2 v[2][4];
         row_unpack<DT>(cur, v);
+        float scale = hc;                            // 1 / sqrt(D) of H and the norm's factor: linear, so once at the end
         if constexpr (NORM) {
             float2 q = make_float2(0.f, 0.f);
+            const float *w = wts + (step < q_steps ? 0 : D);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q = fma2(v[s][i], v[s][i], q);
+                for (int i = 0; i < 2; ++i) {
+                    const float4 f = row_weights(w, s, i, jj, lanes);
+                    q = fma2(v[s][2 * i], v[s][2 * i], q);
+                    q = fma2(v[s][2 * i + 1], v[s][2 * i + 1], q);
+                    v[s][2 * i] = mul2(v[s][2 * i], make_float2(f.x, f.y));
+                    v[s][2 * i + 1] = mul2(v[s][2 * i + 1], make_float2(f.z, f.w));
+                }
             const float sum = row_sum<LANES>(j < lanes ? q.x + q.y : 0.f);
-            const float r = rsqrtf(sum / (float)D + a.eps);
-            const float *w = wts + (h < a.t[0].heads ? 0 : D);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    v[s][i] = mul2(mul2(v[s][i], make_float2(r, r)), *(const float2 *)(w + s * half + 8 * jj + 2 * i));
+            scale *= rsqrtf(sum * inv_d + a.eps);
         }
-        if (HAD && !NORM && a.inverse) row_hadamard<LANES>(v, j, lanes, hc);
+        if (HAD && !NORM && a.inverse) row_hadamard<LANES>(v, j, lanes);
         row_rotate(v, turn, mode, partner);
-        if (HAD && (NORM || !a.inverse)) row_hadamard<LANES>(v, j, lanes, hc);
-        if (mine && h < heads) row_store<DT>(h < a.t[0].heads ? a.t[0].y : a.t[1].y, row(h, true), half, v);
+        if (HAD && (NORM || !a.inverse)) row_hadamard<LANES>(v, j, lanes);
+        if (HAD || NORM) row_scale(v, scale);
+        if (on) row_store<DT>(out, half * SIZE, v);
+        if (step + 1 == q_steps) {
+            if (step + 1 < steps) start_out(a.t[1]);
+        } else {
+            out += out_step;
+        }
     }
 }
 
-// Gradient of norm and rotation, the same layout.  The first `q_blocks` blocks serve the queries, the others the keys;
-// a block walks over tiles of tb tokens and keeps its share of the weights' gradient in registers until the end.
-template <int DT, bool HAD, int LANES>
-__global__ void __launch_bounds__(kRowThreads)
-norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int tb, int mode, int q_blocks)
+// Gradient of norm and rotation, the same layout of a row.  The first `q_blocks` blocks serve the queries, the others the
+// keys.  A warp takes whole tokens (per = 32 / LANES / tokens-of-a-warp groups each) and needs no other warp until the
+// end, where the block's share of the weights' gradient, in registers so far, is added up: with barriers around the
+// table of cos and sin the blocks stood still for a fifth of the time.  Registers are what limits it: the next row comes
+// by cp.async into a slot of shared memory that its own thread alone reads, x is read from there once for each of its
+// three uses, and for split pairs cos and sin stay in shared memory as well.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src)
 {
-    extern __shared__ float2 tab[];                  // [tb][D / 2], at the end [groups][D] floats
-    __shared__ float wts[kMaxHeadDim];
-    constexpr int GROUPS = kRowThreads / LANES;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t from)   // volatile: not kept in registers between two uses
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+    return v;
+}
+// Vector s of a row in its slot, as fp32.
+template <int DT>
+__device__ __forceinline__ void slot_vector(uint32_t from, int s, float2 (&v)[4])
+{
+    constexpr int VECS = DT == B200HT_F32 ? 2 : 1;
+    if constexpr (DT == B200HT_F32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 r = load_shared16(from + (s * VECS + i) * kRowThreads * 16);
+            v[2 * i] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+            v[2 * i + 1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
+        }
+    } else {
+        const uint4 r = load_shared16(from + s * kRowThreads * 16);
+        v[0] = unpack2<DT>(r.x);
+        v[1] = unpack2<DT>(r.y);
+        v[2] = unpack2<DT>(r.z);
+        v[3] = unpack2<DT>(r.w);
+    }
+}
+constexpr int kRowSlots = 2;   // 3 or 4 measured slower in 16 bits (108 us for 97 at 16384 x 40 x 128)
+template <int DT>
+constexpr int row_slot_bytes() { return kRowThreads * 16 * 4 * (DT == B200HT_F32 ? 2 : 1); }   // x and g, two vectors each
+
+template <int DT, bool HAD, int LANES, int MODE>
+__global__ void __launch_bounds__(kRowThreads, DT == B200HT_F32 ? 2 : 3)
+norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int per_k, int q_blocks)
+{
+    extern __shared__ __align__(16) unsigned char smem[];   // slots of rows, the warps' tables; at the end [groups][D] floats
+    __shared__ __align__(16) float wts[kMaxHeadDim];
+    constexpr int GROUPS = kRowThreads / LANES, SIZE = DT == B200HT_F32 ? 4 : 2, VECS = DT == B200HT_F32 ? 2 : 1;
+    constexpr int SLOT = row_slot_bytes<DT>(), WARPS = kRowThreads / 32;
     const int D = a.D, half = D / 2, lanes = D / 16;
     const int which = (int)blockIdx.x < q_blocks ? 0 : 1;
-    const int block = which ? (int)blockIdx.x - q_blocks : (int)blockIdx.x;
-    const int blocks = which ? (int)gridDim.x - q_blocks : q_blocks;
     const RotTensor &t = a.t[which];
-    const int group = threadIdx.x / LANES, j = threadIdx.x % LANES, jj = j < lanes ? j : 0;
-    const int per = GROUPS / tb, tk = group / per, h0 = group - tk * per;
+    const int per = which ? per_k : per_q;                  // groups of one token
+    const int tokens = 32 / LANES / per;                    // tokens of a warp
+    const int warp = threadIdx.x >> 5, group = threadIdx.x / LANES, j = threadIdx.x % LANES, jj = j < lanes ? j : 0;
+    const int tk = group % (32 / LANES) / per, h0 = group % per;
     const int steps = (t.heads + per - 1) / per;
-    const int partner = row_partner(mode, j, a.pairs);
+    const int partner = row_partner(MODE, j, a.pairs);
     const float hc = HAD ? rsqrtf((float)D) : 1.f, inv_d = 1.f / (float)D;
+    const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+    float2 *tab = (float2 *)(smem + kRowSlots * SLOT) + warp * tokens * half;
     pdl_launch_dependents();
     pdl_wait();
-    for (int i = threadIdx.x; i < D; i += kRowThreads) wts[i] = rot_weight<DT>(a, t.w, i);
+    fill_weights<DT>(wts, a, t.w, D, lanes);
+    __syncthreads();
 
     float2 dw[2][4];
 #pragma unroll
@@ -536,59 +633,131 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int tb, int mode,
 #pragma unroll
         for (int i = 0; i < 4; ++i) dw[s][i] = make_float2(0.f, 0.f);
 
-    for (long long token0 = (long long)block * tb; token0 < a.tokens; token0 += (long long)blocks * tb) {
-        const int token = (int)token0 + tk;
-        const bool mine = token < a.tokens && j < lanes;
-        RowRaw<DT> nx = {}, ng = {};
-        if (mine && h0 < t.heads) {
-            row_load<DT>(nx, t.x, token * t.x_tok + h0 * t.x_head + 8 * j, half);
-            row_load<DT>(ng, t.g, token * t.g_tok + h0 * t.g_head + 8 * j, half);
+    // the rows on their way: kRowSlots - 1 steps ahead of the one at work
+    const long long first = ((long long)(which ? (int)blockIdx.x - q_blocks : (int)blockIdx.x) * WARPS + warp) * tokens;
+    const long long stride = (long long)(which ? (int)gridDim.x - q_blocks : q_blocks) * WARPS * tokens;
+    const long long x_step = per * t.x_head * SIZE, g_step = per * t.g_head * SIZE, y_step = per * t.y_head * SIZE;
+    const unsigned char *fx, *fg;
+    long long f_first = first;
+    int f_step = 0, f_left, slot = 0;
+    auto row = [&]() {
+        const long long token = f_first + tk;
+        f_left = token < a.tokens && j < lanes ? t.heads - h0 : 0;
+        fx = (const unsigned char *)t.x + (token * t.x_tok + h0 * t.x_head + 8 * j) * SIZE;
+        fg = (const unsigned char *)t.g + (token * t.g_tok + h0 * t.g_head + 8 * j) * SIZE;
+    };
+    auto fetch = [&](int to_slot) {
+        if (f_left > 0) {
+            const uint32_t to = mine_s + to_slot * SLOT;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < VECS; ++i) {
+                    copy_async16(to + (s * VECS + i) * kRowThreads * 16, fx + s * half * SIZE + 16 * i);
+                    copy_async16(to + ((2 + s) * VECS + i) * kRowThreads * 16, fg + s * half * SIZE + 16 * i);
+                }
         }
-        __syncthreads();
-        fill_turns(tab, a, (int)token0, tb);   // a.inverse is set: the gradient turns back
-        __syncthreads();
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        if (++f_step == steps) {
+            f_step = 0;
+            f_first += stride;
+            row();
+        } else {
+            fx += x_step;
+            fg += g_step;
+            f_left -= per;
+        }
+    };
+    row();
+#pragma unroll
+    for (int i = 0; i + 1 < kRowSlots; ++i) fetch(i);
+    for (long long token0 = first; token0 < a.tokens; token0 += stride) {
+        __syncwarp();
+        fill_turns<32, MODE == kPairsHalves>(tab, a, token0, tokens);   // a.inverse is set: the gradient turns back
+        __syncwarp();
         RowTurn turn;
-        row_turn(turn, tab + tk * half, mode, jj, D, a.pairs);
-        int h = h0;
-        for (int step = 0; step < steps; ++step, h += per) {
-            float2 x[2][4], g[2][4];
-            row_unpack<DT>(nx, x);
-            row_unpack<DT>(ng, g);
-            const bool on = mine && h < t.heads;
-            if (mine && h + per < t.heads) {
-                row_load<DT>(nx, t.x, token * t.x_tok + (h + per) * t.x_head + 8 * j, half);
-                row_load<DT>(ng, t.g, token * t.g_tok + (h + per) * t.g_head + 8 * j, half);
+        if (MODE != kPairsHalves) row_turn(turn, tab + tk * half, MODE, jj, D, a.pairs);
+        const uint32_t turns = (uint32_t)__cvta_generic_to_shared(tab + tk * half) + jj * 32;
+        const long long token = token0 + tk;
+        int left = token < a.tokens && j < lanes ? t.heads - h0 : 0;
+        unsigned char *y = (unsigned char *)t.y + (token * t.y_tok + h0 * t.y_head + 8 * j) * SIZE;
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            fetch(slot == 0 ? kRowSlots - 1 : slot - 1);
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kRowSlots - 1) : "memory");
+            const bool on = left > 0;
+            const uint32_t from_x = mine_s + slot * SLOT, from_g = from_x + 2 * VECS * kRowThreads * 16;
+            slot = slot + 1 == kRowSlots ? 0 : slot + 1;
+            float2 g[2][4];
+            slot_vector<DT>(from_g, 0, g[0]);
+            slot_vector<DT>(from_g, 1, g[1]);
+            if (HAD) row_hadamard<LANES>(g, j, lanes);
+            if constexpr (MODE == kPairsHalves) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 c = load_shared16(turns + 16 * i), sn = load_shared16(turns + half * 4 + 16 * i);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 ce = make_float2(__uint_as_float(e ? c.z : c.x), __uint_as_float(e ? c.w : c.y));
+                        const float2 se = make_float2(__uint_as_float(e ? sn.z : sn.x), __uint_as_float(e ? sn.w : sn.y));
+                        const float2 u = g[0][2 * i + e], v = g[1][2 * i + e];
+                        g[0][2 * i + e] = sub2(mul2(u, ce), mul2(v, se));
+                        g[1][2 * i + e] = fma2(v, ce, mul2(u, se));
+                    }
+                }
+            } else {
+                row_rotate(g, turn, MODE, partner);
             }
-            if (HAD) row_hadamard<LANES>(g, j, lanes, hc);
-            row_rotate(g, turn, mode, partner);
             float2 q = make_float2(0.f, 0.f), d = make_float2(0.f, 0.f);
-            float2 gw[2][4];
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 2; ++s) {
+                float2 x[4];
+                slot_vector<DT>(from_x, s, x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    q = fma2(x[s][i], x[s][i], q);
-                    gw[s][i] = mul2(g[s][i], *(const float2 *)(wts + s * half + 8 * jj + 2 * i));
-                    d = fma2(x[s][i], gw[s][i], d);
-                }
+                for (int i = 0; i < 4; ++i) q = fma2(x[i], x[i], q);
+            }
             const float sum = row_sum<LANES>(j < lanes ? q.x + q.y : 0.f);
-            const float dot = row_sum<LANES>(j < lanes ? d.x + d.y : 0.f);
-            const float r = rsqrtf(sum * inv_d + a.eps);
-            // dx = r (gw - h mean(gw h)), h = x r
-            const float k = -r * r * dot * inv_d;
+            const float r = rsqrtf(sum * inv_d + a.eps), rc = r * hc;
+            // dw += g h with h = x r; then g becomes g w
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 2; ++s) {
+                float2 x[4];
+                slot_vector<DT>(from_x, s, x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (on) dw[s][i] = fma2(g[s][i], mul2(x[s][i], make_float2(r, r)), dw[s][i]);
-                    gw[s][i] = mul2(fma2(x[s][i], make_float2(k, k), gw[s][i]), make_float2(r, r));
+                for (int i = 0; i < 2; ++i) {
+                    const float4 f = row_weights(wts, s, i, jj, lanes);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float2 &gi = g[s][2 * i + e];
+                        const float2 xi = x[2 * i + e];
+                        if (on) dw[s][2 * i + e] = fma2(mul2(gi, xi), make_float2(rc, rc), dw[s][2 * i + e]);
+                        gi = mul2(gi, e ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+                        d = fma2(xi, gi, d);
+                    }
                 }
-            if (on) row_store<DT>(t.y, token * t.y_tok + h * t.y_head + 8 * j, half, gw);
+            }
+            const float dot = row_sum<LANES>(j < lanes ? d.x + d.y : 0.f);
+            // dx = r (gw - h mean(gw h)) = r gw - x r^3 mean(gw x)
+            const float k = -(r * r) * (rc * dot * inv_d);
+            if (on) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    float2 x[4];
+                    slot_vector<DT>(from_x, s, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        g[s][i] = fma2(x[i], make_float2(k, k), mul2(g[s][i], make_float2(rc, rc)));
+                }
+                row_store<DT>(y, half * SIZE, g);
+            }
+            y += y_step;
+            left -= per;
         }
     }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 
     __syncthreads();
-    float *rows = (float *)tab;
+    float *rows = (float *)smem;
     if (j < lanes)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -643,26 +812,27 @@ static int launch_any(const RotArgs &a, bool had, cudaStream_t st)
                : launch_pdl(rotary_any_kernel<DT, NORM, false>, grid, block, 0, st, a);
 }
 
-// Blocks of the gradient kernel that serve the queries and the keys: shares of the rows, at least one each where there
-// are rows.  `most` bounds the sum (the size of the workspace goes by it).
+// Blocks of the gradient kernel that serve the queries and the keys: shares of the work, at least one each where there
+// is any.  `most` bounds the sum (the size of the workspace goes by it).
 struct GradBlocks {
     int q, k;
 };
-static GradBlocks grad_blocks(long long q_rows, long long k_rows, long long rows_per_block, int most)
+static GradBlocks grad_blocks(double q_work, double k_work, double work_per_block, int most)
 {
-    const long long want = (q_rows + k_rows + rows_per_block - 1) / rows_per_block;
-    const long long n = want < most ? want : most;
+    const double want = (q_work + k_work) / work_per_block;
+    const int n = want < most ? (int)want + 1 : most;
     GradBlocks b{0, 0};
-    if (q_rows + k_rows == 0) return b;
-    b.q = q_rows ? (int)(n * q_rows / (q_rows + k_rows)) : 0;
-    if (q_rows && b.q < 1) b.q = 1;
-    b.k = k_rows ? (int)(n - b.q) : 0;
-    if (k_rows && b.k < 1) b.k = 1;
+    if (q_work > 0) {
+        b.q = k_work > 0 ? (int)(n * (q_work / (q_work + k_work)) + 0.5) : n;
+        if (b.q < 1) b.q = 1;
+    }
+    if (k_work > 0) b.k = n - b.q > 1 ? n - b.q : 1;
     return b;
 }
 // Blocks of a gradient launch at most (one more may come from rounding up).  They do not go by the device's number of
 // SMs, so that the order of the sums goes by the sizes alone.
-constexpr int kGradBlocks = 148 * 8, kRowGradBlocks = 148 * 3;
+constexpr int kGradBlocks = 148 * 8;
+constexpr int row_grad_blocks(int dtype) { return 148 * (dtype == B200HT_F32 ? 2 : 3); }   // one wave of resident blocks
 
 static int check_rot_common(const RotArgs &a, int dtype, int flags, const unsigned char *axis_of_pair, int n_axes)
 {
@@ -678,8 +848,9 @@ static int check_rot_common(const RotArgs &a, int dtype, int flags, const unsign
             if (axis_of_pair[i] >= n_axes) return B200HT_ERR_SIZE;
     return 0;
 }
-static void fill_rot_common(RotArgs &a, int flags, const unsigned char *axis_of_pair)
+static void fill_rot_common(RotArgs &a, int flags, const unsigned char *axis_of_pair, int n_axes)
 {
+    a.n_axes = n_axes;
     a.interleaved = (flags & B200HT_ROT_INTERLEAVED) ? 1 : 0;
     a.inverse = (flags & B200HT_ROT_INVERSE) ? 1 : 0;
     a.pos64 = (flags & B200HT_ROT_POS64) ? 1 : 0;
@@ -715,18 +886,17 @@ static int row_mode(const RotArgs &a, int dtype, bool grad)
     return a.pairs % 8 == 0 && 4 * a.pairs <= a.D ? kPairsInFirstHalf : -1;
 }
 
-// Tokens of a block: as many as keep its groups busy (the last step of the walk over the heads may leave some idle)
-// with several rows a group, so that cos and sin and the start of the block are shared; one where there are few tokens
-// and all SMs can have a block of their own.
-static int row_tokens(int groups, int heads, int tokens)
+// Tokens of a block.  Few tokens: one, so that all SMs have a block.  Else as many as leave the fewest groups idle in
+// the last step of each walk over the heads, with several rows a group to share cos and sin and the block's start.
+static int row_tokens(int groups, int q_heads, int k_heads, int tokens)
 {
     if (tokens <= 2 * sm_count()) return 1;
     int best = 1;
     double best_use = 0;
     for (int tb = 1; tb <= groups && tb <= 16; tb *= 2) {
-        const int per = groups / tb, steps = (heads + per - 1) / per;
-        if (steps > 8 && best_use > 0) break;
-        const double use = (double)heads / (per * steps) * steps / (steps + 0.5);
+        const int per = groups / tb, steps = (q_heads + per - 1) / per + (k_heads + per - 1) / per;
+        if (steps > 12 && best_use > 0) break;
+        const double use = (double)(q_heads + k_heads) / (per * (steps + 0.5));
         if (use > best_use) { best_use = use; best = tb; }
     }
     return best;
@@ -735,7 +905,7 @@ static int row_tokens(int groups, int heads, int tokens)
 template <int DT, bool NORM, int LANES>
 static int launch_rows(const RotArgs &a, bool had, int mode, cudaStream_t st)
 {
-    const int tb = row_tokens(kRowThreads / LANES, a.t[0].heads + a.t[1].heads, a.tokens);
+    const int tb = row_tokens(kRowThreads / LANES, a.t[0].heads, a.t[1].heads, a.tokens);
     const size_t smem = (size_t)tb * (a.D / 2) * sizeof(float2) + (NORM ? (size_t)2 * a.D * sizeof(float) : 0);
     const dim3 grid((unsigned)((a.tokens + tb - 1) / tb)), block(kRowThreads);
     return had ? launch_pdl(rotary_row_kernel<DT, NORM, true, LANES>, grid, block, smem, st, a, tb, mode)
@@ -757,31 +927,54 @@ static int launch_rotary(const RotArgs &a, bool norm, bool had, cudaStream_t st)
     return norm ? launch_forward<DT, true>(a, had, DT, st) : launch_forward<DT, false>(a, had, DT, st);
 }
 
+template <int DT, int LANES, int MODE>
+static int launch_row_grad_mode(const RotArgs &a, bool had, GradBlocks *b, cudaStream_t st)
+{
+    // groups of a warp for one token: all of them, fewer where the heads would leave some idle
+    auto per = [](int heads) {
+        int best = 32 / LANES, waste = 1 << 30;
+        for (int p = 32 / LANES; p >= 1; p /= 2) {
+            const int w = (heads + p - 1) / p * p - heads;
+            if (w < waste) { waste = w; best = p; }
+        }
+        return best;
+    };
+    const int per_q = per(a.t[0].heads), per_k = per(a.t[1].heads);
+    // a token costs its steps and, for cos and sin, about as much as one and a half more; a block has eight warps
+    auto work = [&](int heads, int per) {
+        return heads ? (double)a.tokens * (((heads + per - 1) / per) + 1.5) / (32 / LANES / per) : 0.;
+    };
+    const double q_work = work(a.t[0].heads, per_q), k_work = work(a.t[1].heads, per_k);
+    *b = grad_blocks(q_work, k_work, kRowThreads / 32, row_grad_blocks(DT));
+    if (b->q + b->k == 0) return 0;
+    // the sums at the end ([groups][D] floats, 16 KB at most) take the place of the slots of rows (32 KB at least)
+    const int tokens = 32 / LANES / (per_q < per_k ? per_q : per_k);
+    const size_t smem = kRowSlots * row_slot_bytes<DT>() + (size_t)(kRowThreads / 32) * tokens * (a.D / 2) * sizeof(float2);
+    const int rc = had ? ensure_dyn_smem((const void *)norm_rotary_row_grad_kernel<DT, true, LANES, MODE>, (int)smem)
+                       : ensure_dyn_smem((const void *)norm_rotary_row_grad_kernel<DT, false, LANES, MODE>, (int)smem);
+    if (rc) return rc;
+    const dim3 grid((unsigned)(b->q + b->k)), block(kRowThreads);
+    return had ? launch_pdl(norm_rotary_row_grad_kernel<DT, true, LANES, MODE>, grid, block, smem, st, a, per_q, per_k, b->q)
+               : launch_pdl(norm_rotary_row_grad_kernel<DT, false, LANES, MODE>, grid, block, smem, st, a, per_q, per_k, b->q);
+}
+
 template <int DT, int LANES>
 static int launch_row_grad(const RotArgs &a, bool had, int mode, GradBlocks *b, cudaStream_t st)
 {
-    constexpr int groups = kRowThreads / LANES;
-    const int tb = row_tokens(groups, a.t[0].heads > a.t[1].heads ? a.t[0].heads : a.t[1].heads, a.tokens);
-    const long long q_rows = (long long)a.tokens * a.t[0].heads, k_rows = (long long)a.tokens * a.t[1].heads;
-    *b = grad_blocks(q_rows, k_rows, groups, kRowGradBlocks);
-    if (b->q + b->k == 0) return 0;
-    const size_t table = (size_t)tb * (a.D / 2) * sizeof(float2), rows = (size_t)groups * a.D * sizeof(float);
-    const dim3 grid((unsigned)(b->q + b->k)), block(kRowThreads);
-    const size_t smem = table > rows ? table : rows;
-    return had ? launch_pdl(norm_rotary_row_grad_kernel<DT, true, LANES>, grid, block, smem, st, a, tb, mode, b->q)
-               : launch_pdl(norm_rotary_row_grad_kernel<DT, false, LANES>, grid, block, smem, st, a, tb, mode, b->q);
+    if (mode == kPairsHalves) return launch_row_grad_mode<DT, LANES, kPairsHalves>(a, had, b, st);
+    if (mode == kPairsNeighbour) return launch_row_grad_mode<DT, LANES, kPairsNeighbour>(a, had, b, st);
+    return launch_row_grad_mode<DT, LANES, kPairsInFirstHalf>(a, had, b, st);
 }
 
 template <int DT>
 static int launch_norm_grad(RotArgs &a, bool had, void *dwq, void *dwk, cudaStream_t st)
 {
-    const long long q_rows = (long long)a.tokens * a.t[0].heads, k_rows = (long long)a.tokens * a.t[1].heads;
     const int mode = row_mode(a, DT, true);
     a.inverse = 1;
     GradBlocks b{0, 0};
     int rc = 0;
     if (mode < 0) {
-        b = grad_blocks(q_rows, k_rows, kAnyWarps, kGradBlocks);
+        b = grad_blocks((double)a.tokens * a.t[0].heads, (double)a.tokens * a.t[1].heads, kAnyWarps, kGradBlocks);
         if (b.q + b.k) {
             const dim3 grid((unsigned)(b.q + b.k)), block(32 * kAnyWarps);
             rc = had ? launch_pdl(norm_rotary_any_grad_kernel<DT, true>, grid, block, 0, st, a, b.q)
@@ -829,7 +1022,7 @@ extern "C" int b200ht_rotary_qk(const void *q, const void *k, void *q_out, void 
     a.pos_tok = pos_token_stride;
     a.inv_freq = inv_freq;
     a.eps = eps;
-    fill_rot_common(a, flags, axis_of_pair);
+    fill_rot_common(a, flags, axis_of_pair, n_axes);
     rc = check_rot_pointers(a, dtype, flags);
     if (rc) return rc;
     rc = check_device();
@@ -884,7 +1077,7 @@ extern "C" int b200ht_norm_rotary_qk_backward(const void *dq_out, const void *dk
     a.inv_freq = inv_freq;
     a.eps = eps;
     a.partial = (float *)workspace;
-    fill_rot_common(a, flags, axis_of_pair);
+    fill_rot_common(a, flags, axis_of_pair, n_axes);
     if (tokens > 0) {
         rc = check_rot_pointers(a, dtype, flags);
         if (rc) return rc;

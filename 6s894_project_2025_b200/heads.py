@@ -10,17 +10,17 @@ libb200ht.so (fp32, angles reduced in fp64, one rounding on the store); there is
 """
 from __future__ import annotations
 
-import ctypes
 import functools
+import struct
 
 import torch
 
 from . import _lib
-from .ops import _DT, _is_pow2, _stream_ptr
+from .ops import _DT, _is_pow2, _on_device, _stream_ptr
 
-_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
-_Strides8 = ctypes.c_longlong * 8
-_Strides12 = ctypes.c_longlong * 12
+_INTS = (torch.int32, torch.int64)
+_strides8 = struct.Struct("8q").pack
+_strides12 = struct.Struct("12q").pack
 
 
 @functools.lru_cache(maxsize=64)
@@ -45,16 +45,18 @@ def axis_table(sections: tuple[int, ...], axis_order: str, pairs: int) -> bytes:
 
 
 def _check_heads(x: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
-    if x.dim() != 3 or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2]:
+    sx, sl = x.shape, like.shape
+    if len(sx) != 3 or sx[0] != sl[0] or sx[2] != sl[2]:
         raise RuntimeError(f"rotary: expected {what} of shape (tokens, heads, head_dim) like the queries")
     if x.dtype != like.dtype or x.device != like.device:
         raise RuntimeError(f"rotary: {what} must have the queries' dtype and device")
-    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+    return x if x.stride(2) == 1 else x.contiguous()
 
 
 def _check_common(q, positions, inv_freq, sections, axis_order, hadamard):
     """Checks shared by all entry points; returns (head_dim, tokens, pairs, flags, axis table, n_axes, pos strides)."""
-    if q.dtype not in _FLOATS:
+    device = q.device
+    if q.dtype not in _DT:
         raise RuntimeError("rotary: only fp16, bf16 and fp32 are supported")
     if not q.is_cuda:
         raise RuntimeError("rotary: queries and keys must be CUDA tensors")
@@ -65,12 +67,12 @@ def _check_common(q, positions, inv_freq, sections, axis_order, hadamard):
         raise RuntimeError(f"rotary: head_dim must be even and at most 256, got {D}")
     if hadamard and not _is_pow2(D):
         raise RuntimeError(f"rotary: the Hadamard rotation needs a head_dim that is a power of two, got {D}")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.device != q.device:
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.device != device:
         raise RuntimeError("rotary: inv_freq must be a float32 vector on the queries' device")
     pairs = inv_freq.shape[0]
     if pairs < 1 or 2 * pairs > D:
         raise RuntimeError(f"rotary: inv_freq must have 1 to head_dim / 2 entries, got {pairs}")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+    if positions.dtype not in _INTS or positions.device != device:
         raise RuntimeError("rotary: positions must be int32 or int64 on the queries' device")
     if sections is None:
         table, n_axes = None, 1
@@ -145,8 +147,8 @@ def _run(q, k, q_weight, k_weight, eps, positions, inv_freq, sections, axis_orde
             raise RuntimeError("rotary: in place, queries and keys must not share memory with themselves or each other")
         qo, ko = q, k
     else:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     if interleaved:
         flags |= _lib.ROT_INTERLEAVED
     if inverse:
@@ -155,15 +157,13 @@ def _run(q, k, q_weight, k_weight, eps, positions, inv_freq, sections, axis_orde
     hk = 0 if k is None else k.shape[1]
     if tokens and q.shape[1] + hk:
         kk, kko = (q, qo) if k is None else (k, ko)   # no keys: the pointers of no head are never read
-        strides = _Strides8(q.stride(0), q.stride(1), kk.stride(0), kk.stride(1), qo.stride(0), qo.stride(1),
-                            kko.stride(0), kko.stride(1))
-        lib = _lib.load()
-        with torch.cuda.device(q.device):
-            rc = lib.b200ht_rotary_qk(q.data_ptr(), kk.data_ptr(), qo.data_ptr(), kko.data_ptr(),
-                                      None if q_weight is None else q_weight.data_ptr(),
-                                      None if k_weight is None else k_weight.data_ptr(), eps, tokens, q.shape[1], hk, D,
-                                      strides, _DT[q.dtype], positions.data_ptr(), pa, pt, n_axes, table,
-                                      inv_freq.data_ptr(), pairs, flags, _stream_ptr(q.device))
+        with _on_device(q.device):
+            rc = _lib.load().b200ht_rotary_qk(
+                q.data_ptr(), kk.data_ptr(), qo.data_ptr(), kko.data_ptr(),
+                None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+                tokens, q.shape[1], hk, D, _strides8(*q.stride()[:2], *kk.stride()[:2], *qo.stride()[:2], *kko.stride()[:2]),
+                _DT[q.dtype], positions.data_ptr(), pa, pt, n_axes, table, inv_freq.data_ptr(), pairs, flags,
+                _stream_ptr(q.device))
         _lib.check(rc, "b200ht_rotary_qk")
     return qo, ko
 
@@ -223,19 +223,18 @@ def norm_rotary_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
     if interleaved:
         flags |= _lib.ROT_INTERLEAVED
     inv_freq = inv_freq.contiguous()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    dw = torch.empty((2, D), dtype=q_weight.dtype, device=q.device)
-    strides = _Strides12(dq_out.stride(0), dq_out.stride(1), dk_out.stride(0), dk_out.stride(1), q.stride(0), q.stride(1),
-                         k.stride(0), k.stride(1), dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1))
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    strides = _strides12(*dq_out.stride()[:2], *dk_out.stride()[:2], *q.stride()[:2], *k.stride()[:2], *dq.stride()[:2],
+                         *dk.stride()[:2])
     lib = _lib.load()
-    ws = torch.empty(int(lib.b200ht_norm_rotary_qk_backward_workspace_bytes(D)), dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        rc = lib.b200ht_norm_rotary_qk_backward(dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
-                                                q_weight.data_ptr(), k_weight.data_ptr(), float(eps), dq.data_ptr(),
-                                                dk.data_ptr(), dw[0].data_ptr(), dw[1].data_ptr(), tokens, q.shape[1],
-                                                k.shape[1], D, strides, _DT[q.dtype], positions.data_ptr(), pa, pt, n_axes,
-                                                table, inv_freq.data_ptr(), pairs, flags, ws.data_ptr(), ws.numel(),
-                                                _stream_ptr(q.device))
+    ws = torch.empty(lib.b200ht_norm_rotary_qk_backward_workspace_bytes(D), dtype=torch.uint8, device=q.device)
+    with _on_device(q.device):
+        rc = lib.b200ht_norm_rotary_qk_backward(
+            dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+            float(eps), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), tokens, q.shape[1], k.shape[1], D,
+            strides, _DT[q.dtype], positions.data_ptr(), pa, pt, n_axes, table, inv_freq.data_ptr(), pairs, flags,
+            ws.data_ptr(), ws.numel(), _stream_ptr(q.device))
     _lib.check(rc, "b200ht_norm_rotary_qk_backward")
-    return dq, dk, dw[0], dw[1]
+    return dq, dk, dqw, dkw

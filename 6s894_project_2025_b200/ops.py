@@ -13,6 +13,7 @@ rejected exactly as the reference rejects them.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -26,8 +27,22 @@ def _is_pow2(v: int) -> bool:
     return v > 0 and (v & (v - 1)) == 0
 
 
+# the raw handle without a Stream object around it (2 us less a call), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(device: torch.device):
+    """A context in which ``device`` is the current one; changes nothing (and costs nothing) where it already is."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def sign_mask(signs: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:

@@ -129,10 +129,9 @@ def norm_rotary_qk_backward_op(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tens
                                inv_freq: torch.Tensor, eps: float = 1e-6, sections: Optional[Sequence[int]] = None,
                                axis_order: str = "blocks", interleaved: bool = False, hadamard: bool = False
                                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    dq, dk, dqw, dkw = heads.norm_rotary_qk_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, eps=eps,
-                                                     sections=sections, axis_order=axis_order, interleaved=interleaved,
-                                                     hadamard=hadamard)
-    return dq, dk, dqw, dkw.clone()   # an operator's results may not share memory
+    return heads.norm_rotary_qk_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, eps=eps,
+                                         sections=sections, axis_order=axis_order, interleaved=interleaved,
+                                         hadamard=hadamard)
 
 
 @norm_rotary_qk_backward_op.register_fake
