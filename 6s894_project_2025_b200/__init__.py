@@ -8,6 +8,10 @@ from .heads import (  # noqa: F401
     norm_rotary_qk_backward,
     rotary_qk,
 )
+from .lora import (  # noqa: F401
+    lora_ht_gemm,
+    lora_ht_gemv,
+)
 from .ops import (  # noqa: F401
     HostPipeline,
     device_status,
@@ -33,6 +37,8 @@ __all__ = [
     "fused_ht_gemm",
     "fused_ht_gemv",
     "fused_gemm_workspace_bytes",
+    "lora_ht_gemm",
+    "lora_ht_gemv",
     "rotary_qk",
     "norm_rotary_qk",
     "norm_rotary_qk_backward",

@@ -35,6 +35,10 @@ EXPORTS = (
     "b200ht_rotary_qk",
     "b200ht_norm_rotary_qk_backward",
     "b200ht_norm_rotary_qk_backward_workspace_bytes",
+    "b200ht_lora_gemm",
+    "b200ht_lora_gemm_workspace_bytes",
+    "b200ht_lora_gemv",
+    "b200ht_lora_gemv_workspace_bytes",
     "b200ht_ipc_export",
     "b200ht_ipc_open",
     "b200ht_ipc_close",
@@ -86,6 +90,15 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.b200ht_norm_rotary_qk_backward.argtypes = [vp, vp, vp, vp, vp, vp, f, vp, vp, vp, vp, i, i, i, i,
                                                    vp, i, vp, ll, ll, i, ctypes.c_char_p, vp, i, i, vp,
                                                    ctypes.c_size_t, vp]
+    sz = ctypes.c_size_t
+    lib.b200ht_lora_gemm_workspace_bytes.restype = sz
+    lib.b200ht_lora_gemm_workspace_bytes.argtypes = [i, i, i, i]
+    lib.b200ht_lora_gemm.restype = i
+    lib.b200ht_lora_gemm.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, f, vp, vp, sz, vp]
+    lib.b200ht_lora_gemv_workspace_bytes.restype = sz
+    lib.b200ht_lora_gemv_workspace_bytes.argtypes = [i, i, i]
+    lib.b200ht_lora_gemv.restype = i
+    lib.b200ht_lora_gemv.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, vp, sz, vp]
     lib.b200ht_ipc_export.restype = i
     lib.b200ht_ipc_export.argtypes = [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_ulonglong)]
     lib.b200ht_ipc_open.restype = i

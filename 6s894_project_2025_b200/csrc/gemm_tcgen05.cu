@@ -16,10 +16,16 @@
 //               shared memory and written by TMA (32 rows x 128 bytes per op)
 // Every mbarrier wait is time-limited; on expiry the CTA drains and exits and
 // the device status word carries B200HT_ERR_TIMEOUT.
+//
+// With adapters (ADAPT, b200ht_lora_gemm) the K loop of a tile is followed by one more stretch per adapter among the
+// tile's 256 tokens: its B matrix (128 * MT rows x rank) against the tokens' low-rank vectors S (256 x rank), into the
+// same accumulator, so the adapters cost rank / K of the contraction, no pass over C, and no second rounding.  The
+// tokens of other adapters are taken out of S in shared memory, by the MMA warp between the copy and the instructions.
 #include <cstdlib>
 #include <mutex>
 
 #include "tc_common.cuh"
+#include "lora.cuh"
 
 namespace b200ht {
 
@@ -131,11 +137,41 @@ __device__ __forceinline__ void tc_tile_coord(int tile, int mt, int nt, TileOrde
     nb = ord.order == 0 ? o : i;
 }
 
-template <int OUT_DT, int LAYOUT, int MT>
+// Kernel argument of the form with adapters; nothing without.
+template <bool ADAPT>
+struct AdaptArgs {};
+template <>
+struct AdaptArgs<true> {
+    CUtensorMap tmB;     // [adapter][M][rank]
+    CUtensorMap tmS;     // [token][rank]
+    const int *tiles;    // kLoraTileInts a 256-token tile: number of its adapters, their numbers, ...
+    const int *index;    // adapter of each token
+    int rank;
+    int row;             // row of B of this launch's first row of C
+};
+
+// Zeroes the rows (128 bytes each) of the 256 x 64 tile at `tile` whose token does not belong to `adapter`; `ids`:
+// adapters of tokens lane, lane + 32, ...  One warp, four rows an instruction.
+__device__ __forceinline__ void tc_mask_rows(uint32_t tile, const int (&ids)[TC_BN / 32], int adapter, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < TC_BN / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 32; r += 4) {
+            const int row = r + (lane >> 3);
+            if (__shfl_sync(0xffffffffu, ids[i], row) != adapter)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(tile + (uint32_t)((i * 32 + row) * 128 + (lane & 7) * 16)),
+                             "r"(0)
+                             : "memory");
+        }
+}
+
+template <int OUT_DT, int LAYOUT, int MT, bool ADAPT>
 __global__ void __launch_bounds__(TcCfg<MT>::THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
                const __grid_constant__ CUtensorMap tmC, int tma_store, void *C, int M, int N, int K, size_t ldc,
-               int ntiles_run, int pdl_mode, TileOrder ord, const float *row_scale, const float *tok_scale, int *status)
+               int ntiles_run, int pdl_mode, TileOrder ord, const float *row_scale, const float *tok_scale, int *status,
+               const __grid_constant__ AdaptArgs<ADAPT> adapt)
 {
     using Cfg = TcCfg<MT>;
     constexpr int STAGES = Cfg::STAGES, STAGE_BYTES = Cfg::STAGE_BYTES, NACC = Cfg::NACC;
@@ -210,6 +246,22 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                     tma_load_2d(sa, &tmW, kb * TC_BK, m0, full_bar(s));
                     tma_load_2d(sa + Cfg::A_BYTES, &tmY, kb * TC_BK, n0, full_bar(s));
                 }
+                if constexpr (ADAPT) {
+                    const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
+                    const int count = __ldcg(mine);
+                    for (int i = 0; i < count && ok; ++i) {
+                        const int adapter = __ldcg(mine + 1 + i);
+                        for (int r = 0; r < adapt.rank; r += TC_BK, ++it) {
+                            const int s = it % STAGES;
+                            const uint32_t ph = (it / STAGES) & 1u;
+                            if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, status)) { ok = false; break; }
+                            mbar_expect_tx(full_bar(s), STAGE_BYTES);
+                            const uint32_t sa = base + s * STAGE_BYTES;
+                            tma_load_3d(sa, &adapt.tmB, r, adapt.row + m0, adapter, full_bar(s));
+                            tma_load_3d(sa + Cfg::A_BYTES, &adapt.tmS, r, n0, 0, full_bar(s));
+                        }
+                    }
+                }
             }
             if (!ok) {
                 // copies already issued still land in this CTA's shared memory: give them time
@@ -224,33 +276,78 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (ADAPT || lane == 0) {   // with adapters the whole warp keeps step: it masks, lane 0 issues
             constexpr uint32_t idesc = umma_idesc_bf16(128, TC_BN);
             uint32_t it = 0, tcount = 0;
             bool ok = true;
             for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x, ++tcount) {
                 const int acc = tcount % NACC;
                 const uint32_t aph = (tcount / NACC) & 1u;
-                if (!mbar_wait(tempty_bar(acc), aph ^ 1u, abort_flag, status)) { ok = false; break; }
-                tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * TC_BN;   // MT == 2: halves at columns 0 and 256
-                for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    const uint32_t ph = (it / STAGES) & 1u;
-                    if (!mbar_wait(full_bar(s), ph, abort_flag, status)) { ok = false; break; }
+                if (lane == 0) {
+                    ok = mbar_wait(tempty_bar(acc), aph ^ 1u, abort_flag, status);
                     tc_fence_after();
-                    const uint32_t sa = base + s * STAGE_BYTES;
-                    const uint64_t bdesc = umma_desc_k_sw128(sa + Cfg::A_BYTES);
+                    for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
+                        const int s = it % STAGES;
+                        const uint32_t ph = (it / STAGES) & 1u;
+                        if (!mbar_wait(full_bar(s), ph, abort_flag, status)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t sa = base + s * STAGE_BYTES;
+                        const uint64_t bdesc = umma_desc_k_sw128(sa + Cfg::A_BYTES);
 #pragma unroll
-                    for (int h = 0; h < MT; ++h) {
-                        const uint64_t adesc = umma_desc_k_sw128(sa + h * 16384);
+                        for (int h = 0; h < MT; ++h) {
+                            const uint64_t adesc = umma_desc_k_sw128(sa + h * 16384);
 #pragma unroll
-                        for (int k = 0; k < TC_BK / 16; ++k)
-                            umma_bf16_ss(d_tmem + h * TC_BN, adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) ? 1u : 0u);
+                            for (int k = 0; k < TC_BK / 16; ++k)
+                                umma_bf16_ss(d_tmem + h * TC_BN, adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) ? 1u : 0u);
+                        }
+                        umma_commit(empty_bar(s));
                     }
-                    umma_commit(empty_bar(s));
                 }
-                if (ok) umma_commit(tfull_bar(acc));
+                if constexpr (ADAPT) {
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    it = __shfl_sync(0xffffffffu, it, 0);
+                    int mb, nb;
+                    tc_tile_coord(tile, mt, nt, ord, mb, nb);
+                    const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
+                    const int count = __ldcg(mine);
+                    int ids[TC_BN / 32];
+                    if (count > 1)
+#pragma unroll
+                        for (int i = 0; i < TC_BN / 32; ++i) {
+                            const int n = nb * TC_BN + i * 32 + lane;
+                            ids[i] = n < N ? __ldcg(adapt.index + n) : -1;
+                        }
+                    for (int i = 0; i < count && ok; ++i) {
+                        const int adapter = __ldcg(mine + 1 + i);
+                        for (int r = 0; r < adapt.rank; r += TC_BK, ++it) {
+                            const int s = it % STAGES;
+                            const uint32_t ph = (it / STAGES) & 1u;
+                            ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, abort_flag, status));
+                            if (!ok) break;
+                            const uint32_t sa = base + s * STAGE_BYTES;
+                            if (count > 1) {   // tokens without an adapter have S = 0 as it is
+                                tc_mask_rows(sa + Cfg::A_BYTES, ids, adapter, lane);
+                                fence_proxy_async();
+                                __syncwarp();
+                            }
+                            if (lane == 0) {
+                                tc_fence_after();
+                                const uint64_t bdesc = umma_desc_k_sw128(sa + Cfg::A_BYTES);
+                                const int ksteps = adapt.rank - r >= TC_BK ? TC_BK / 16 : (adapt.rank - r + 15) / 16;
+#pragma unroll
+                                for (int h = 0; h < MT; ++h) {
+                                    const uint64_t adesc = umma_desc_k_sw128(sa + h * 16384);
+                                    for (int k = 0; k < ksteps; ++k)
+                                        umma_bf16_ss(d_tmem + h * TC_BN, adesc + 2 * k, bdesc + 2 * k, idesc, 1u);
+                                }
+                                umma_commit(empty_bar(s));
+                            }
+                            __syncwarp();
+                        }
+                    }
+                }
+                if (ok && lane == 0) umma_commit(tfull_bar(acc));
             }
         }
         __syncwarp();
@@ -530,6 +627,22 @@ int encode_tmap_bf16_row_groups(CUtensorMap *map, const void *base, uint64_t gro
     });
 }
 
+// [d2][d1][d0] bf16, d0 contiguous (d0 a multiple of 8), box 1 x box1 x 64 with 128-byte swizzle; a box that reaches
+// beyond d0 or d1 is filled with zeros.
+int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1)
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return (int)cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {d0, d1, d2};
+    const cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
+    const cuuint32_t box[3] = {64, box1, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
 // Output map for the TMA-store epilogue: rows x cols of fp32 or bf16, box = 32 rows x 128 bytes, 128-byte swizzle.
 static int encode_tmap_out_2d(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t ld, int dtype)
 {
@@ -545,9 +658,11 @@ static int encode_tmap_out_2d(CUtensorMap *map, const void *base, uint64_t rows,
     });
 }
 
+// `lora`: the adapters, advanced by the caller to the first token and row of this launch (nullptr: none).
 template <int OUT_DT, int LAYOUT, int MT>
 static int launch_tc_mt(const void *Y, const void *W, void *C, int M, int N, int K, size_t ldc, int skip_last_tiles,
-                        int pdl_mode, TileOrder ord, const float *row_scale, const float *tok_scale, cudaStream_t st)
+                        int pdl_mode, TileOrder ord, const float *row_scale, const float *tok_scale, cudaStream_t st,
+                        const LoraGemm *lora)
 {
     using Cfg = TcCfg<MT>;
     CUtensorMap tw, ty;
@@ -564,17 +679,34 @@ static int launch_tc_mt(const void *Y, const void *W, void *C, int M, int N, int
             encode_tmap_out_2d(&tc, C, (uint64_t)M, (uint64_t)N, (uint64_t)ldc, OUT_DT) == 0)
             tma_store = 1;
     }
-    rc = ensure_dyn_smem((const void *)gemm_tc_kernel<OUT_DT, LAYOUT, MT>, Cfg::SMEM_BYTES);
-    if (rc) return rc;
     const int tiles = ((M + Cfg::BM - 1) / Cfg::BM) * ((N + TC_BN - 1) / TC_BN) - skip_last_tiles;
     const int grid = tiles < sm_count() ? tiles : sm_count();
-    return launch_pdl(gemm_tc_kernel<OUT_DT, LAYOUT, MT>, dim3(grid), dim3(Cfg::THREADS), (size_t)Cfg::SMEM_BYTES, st,
-                      tw, ty, tc, tma_store, C, M, N, K, ldc, tiles, pdl_mode, ord, row_scale, tok_scale, status_word_ptr());
+    if (lora) {
+        AdaptArgs<true> ad{};
+        rc = encode_tmap_bf16_stack(&ad.tmB, lora->B, (uint64_t)lora->adapters, (uint64_t)lora->M, (uint64_t)lora->rank, Cfg::BM);
+        if (rc) return rc;
+        rc = encode_tmap_bf16_stack(&ad.tmS, lora->S, 1, (uint64_t)N, (uint64_t)lora->rank, TC_BN);
+        if (rc) return rc;
+        ad.tiles = lora->tiles;
+        ad.index = lora->index;
+        ad.rank = lora->rank;
+        ad.row = lora->row;
+        rc = ensure_dyn_smem((const void *)gemm_tc_kernel<OUT_DT, LAYOUT, MT, true>, Cfg::SMEM_BYTES);
+        if (rc) return rc;
+        return launch_pdl(gemm_tc_kernel<OUT_DT, LAYOUT, MT, true>, dim3(grid), dim3(Cfg::THREADS), (size_t)Cfg::SMEM_BYTES, st,
+                          tw, ty, tc, tma_store, C, M, N, K, ldc, tiles, pdl_mode, ord, row_scale, tok_scale, status_word_ptr(),
+                          ad);
+    }
+    rc = ensure_dyn_smem((const void *)gemm_tc_kernel<OUT_DT, LAYOUT, MT, false>, Cfg::SMEM_BYTES);
+    if (rc) return rc;
+    return launch_pdl(gemm_tc_kernel<OUT_DT, LAYOUT, MT, false>, dim3(grid), dim3(Cfg::THREADS), (size_t)Cfg::SMEM_BYTES, st,
+                      tw, ty, tc, tma_store, C, M, N, K, ldc, tiles, pdl_mode, ord, row_scale, tok_scale, status_word_ptr(),
+                      AdaptArgs<false>{});
 }
 
 template <int OUT_DT, int LAYOUT>
 static int launch_tc(const void *Y, const void *W, void *C, int M, int N, int K, size_t ldc_arg, const float *row_scale,
-                     const float *tok_scale, cudaStream_t st)
+                     const float *tok_scale, cudaStream_t st, const LoraGemm *lora)
 {
     // 256-row or 128-row CTA tiles: whichever needs less time in units of a 128-row tile, counting whole waves
     // over the SMs (a 256-row tile costs two units; 128-row tiles pay about 3 % more for operand traffic).
@@ -616,31 +748,35 @@ static int launch_tc(const void *Y, const void *W, void *C, int M, int N, int K,
     const double cost128 = 1.03 * (double)((tiles128 + sms - 1) / sms);
     const double cost256 = can_split ? 2.0 * (double)(tiles256 / sms) + 1.03 : 2.0 * (double)((tiles256 + sms - 1) / sms);
     const bool big = force_mt ? force_mt == 2 : (tiles256 >= sms && cost256 <= cost128);
-    if (!big) return launch_tc_mt<OUT_DT, LAYOUT, 1>(Y, W, C, M, N, K, ldc, 0, 0, ord, row_scale, tok_scale, st);
+    if (!big) return launch_tc_mt<OUT_DT, LAYOUT, 1>(Y, W, C, M, N, K, ldc, 0, 0, ord, row_scale, tok_scale, st, lora);
     if (can_split && !force_mt) {
         const long in_blocks = rem <= gl ? rem : gl;          // blocks of the rectangle along the grouped dimension
         const long out_blocks = rem <= gl ? 1 : rem / gl;     // ... and along the other one
         const long rows = ord.order == 0 ? in_blocks : out_blocks;   // 256-row blocks
         const long cols = ord.order == 0 ? out_blocks : in_blocks;   // token blocks
         const long row_off = (mt256 - rows) * 256, tok_off = (nt - cols) * TC_BN;
-        int rc = launch_tc_mt<OUT_DT, LAYOUT, 2>(Y, W, C, M, N, K, ldc, (int)rem, 1, ord, row_scale, tok_scale, st);
+        int rc = launch_tc_mt<OUT_DT, LAYOUT, 2>(Y, W, C, M, N, K, ldc, (int)rem, 1, ord, row_scale, tok_scale, st, lora);
         if (rc) return rc;
         const size_t esz = OUT_DT == B200HT_F32 ? 4 : 2;
         const size_t coff = LAYOUT == B200HT_OUT_MN ? (size_t)row_off * ldc + (size_t)tok_off : (size_t)tok_off * ldc + (size_t)row_off;
+        LoraGemm tail;
+        if (lora) tail = lora->at(row_off, tok_off);
         return launch_tc_mt<OUT_DT, LAYOUT, 1>((const unsigned char *)Y + (size_t)tok_off * K * 2,
                                                (const unsigned char *)W + (size_t)row_off * K * 2,
                                                (unsigned char *)C + coff * esz, (int)(M - row_off), (int)(N - tok_off), K, ldc,
                                                0, 2, ord, row_scale ? row_scale + row_off : nullptr,
-                                               tok_scale ? tok_scale + tok_off : nullptr, st);
+                                               tok_scale ? tok_scale + tok_off : nullptr, st, lora ? &tail : nullptr);
     }
-    return launch_tc_mt<OUT_DT, LAYOUT, 2>(Y, W, C, M, N, K, ldc, 0, 0, ord, row_scale, tok_scale, st);
+    return launch_tc_mt<OUT_DT, LAYOUT, 2>(Y, W, C, M, N, K, ldc, 0, 0, ord, row_scale, tok_scale, st, lora);
 }
 
 // `ldc` = leading dimension of C in elements when C is a block of a larger matrix (0: the block is the matrix).
 int launch_gemm_bf16_tcgen05(const void *Y, const void *W, void *C, int M, int N, int K, int out_dtype,
-                             int out_layout, cudaStream_t st, const float *row_scale, const float *tok_scale, size_t ldc)
+                             int out_layout, cudaStream_t st, const float *row_scale, const float *tok_scale, size_t ldc,
+                             const LoraGemm *lora)
 {
     if (K < TC_BK) {
+        if (lora) return B200HT_ERR_SIZE;
         dim3 blk(32, 8), grd((N + 31) / 32, (M + 7) / 8);
         note_launch();
         gemm_bf16_smallk_kernel<<<grd, blk, 0, st>>>((const __nv_bfloat16 *)Y, (const __nv_bfloat16 *)W, C, M, N, K,
@@ -649,12 +785,12 @@ int launch_gemm_bf16_tcgen05(const void *Y, const void *W, void *C, int M, int N
     }
     if (out_dtype == B200HT_F32) {
         return out_layout == B200HT_OUT_MN
-                   ? launch_tc<B200HT_F32, B200HT_OUT_MN>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st)
-                   : launch_tc<B200HT_F32, B200HT_OUT_NM>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st);
+                   ? launch_tc<B200HT_F32, B200HT_OUT_MN>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st, lora)
+                   : launch_tc<B200HT_F32, B200HT_OUT_NM>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st, lora);
     }
     return out_layout == B200HT_OUT_MN
-               ? launch_tc<B200HT_BF16, B200HT_OUT_MN>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st)
-               : launch_tc<B200HT_BF16, B200HT_OUT_NM>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st);
+               ? launch_tc<B200HT_BF16, B200HT_OUT_MN>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st, lora)
+               : launch_tc<B200HT_BF16, B200HT_OUT_NM>(Y, W, C, M, N, K, ldc, row_scale, tok_scale, st, lora);
 }
 
 }  // namespace b200ht

@@ -1,0 +1,136 @@
+"""W . H(X) with low-rank adapters of many requests beside the shared projection.
+
+One batch holds tokens of many requests, each with its own adapter or none; they share the weight W.  The adapters are
+stacked: A (adapters, rank, K) and B (adapters, M, rank), token t has adapter ``index[t]``, and its output gains
+``scaling[a] * B[a] @ (A[a] @ x_t)``.  The adapter sees the token as given, without H, as it was trained beside the
+unrotated weight.  These are serving operators: W and the adapters get no gradient.  The reference has no counterpart.
+
+All arithmetic happens in libb200ht.so, bf16 operands with fp32 sums; there is no CPU path.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .ops import _DT, _is_pow2, _on_device, _stream_ptr, sign_mask
+
+_MAX_COLUMNS = 64   # columns of one decoding call; more go through the contraction
+
+
+def _check(what: str, X, W, A, B, index, scaling, tokens: int, K: int, out_dtype):
+    """Checks shared by both entries; returns (M, adapters, rank, A, B, index, scaling)."""
+    bf16, device = torch.bfloat16, X.device
+    if X.dtype != bf16 or W.dtype != bf16 or A.dtype != bf16 or B.dtype != bf16:
+        raise RuntimeError(f"{what}: X, W, A and B must be bfloat16")
+    if not X.is_cuda or W.device != device or A.device != device or B.device != device or index.device != device:
+        raise RuntimeError(f"{what}: all tensors must be on one CUDA device")
+    if not _is_pow2(K) or K < 64 or K > (1 << 15):
+        raise RuntimeError(f"{what}: the Hadamard size must be a power of two from 64 to 2^15, got {K}")
+    M = W.shape[0]
+    if A.dim() != 3 or B.dim() != 3 or A.shape[2] != K or B.shape[1] != M or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2]:
+        raise RuntimeError(f"{what}: expected A (adapters, rank, {K}) and B (adapters, {M}, rank)")
+    adapters, rank = A.shape[0], A.shape[1]
+    if adapters < 1 or rank < 8 or rank > 128 or rank % 8:
+        raise RuntimeError(f"{what}: the rank must be a multiple of 8 up to 128 (pad with zeros) of at least one adapter, got "
+                           f"{adapters} of rank {rank}")
+    if index.dtype != torch.int32 or index.dim() != 1 or index.shape[0] != tokens:
+        raise RuntimeError(f"{what}: index must be {tokens} int32 entries")
+    if scaling is not None:
+        if scaling.dtype != torch.float32 or scaling.dim() != 1 or scaling.shape[0] != adapters or scaling.device != device:
+            raise RuntimeError(f"{what}: scaling must be {adapters} float32 entries on the tokens' device")
+        scaling = scaling.contiguous()
+    if out_dtype not in (torch.float32, bf16):
+        raise RuntimeError(f"{what}: out_dtype must be float32 or bfloat16")
+    return M, adapters, rank, _rows(A), _rows(B), index.contiguous(), scaling
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x contiguous and on a 16-byte boundary."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _out(what, out, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.device != device or out.data_ptr() % 16:
+        raise RuntimeError(f"{what}: out has the wrong shape, dtype, strides, device or alignment")
+    return out
+
+
+def lora_ht_gemm(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, index: torch.Tensor, *,
+                 scaling: torch.Tensor | None = None, scale: float | None = None, out_dtype: torch.dtype | None = None,
+                 out_layout: str = "mn", out: torch.Tensor | None = None, signs: torch.Tensor | None = None) -> torch.Tensor:
+    """``fused_ht_gemm(X, W)`` plus the adapter of each token, in one contraction.
+
+    ``X`` (N tokens, K), ``W`` (M, K), ``A`` (adapters, rank, K) and ``B`` (adapters, M, rank) are bf16; ``index`` (N
+    int32 entries) names the adapter of each token, any value outside 0 .. adapters - 1 (-1, say) none; ``scaling``
+    (float32, one per adapter) defaults to 1.  The rank is a multiple of 8 up to 128.  ``scale``, ``signs``,
+    ``out_dtype`` (float32 by default), ``out_layout`` and ``out`` as in ``fused_ht_gemm``; scale and signs belong to the
+    transform and do not touch the adapters.  Tokens may come in any order; tokens of one adapter next to each other cost
+    least.  The low-rank vectors are rounded to bf16, as H(X) is, the sums are fp32 and C is rounded once.
+
+    An adapter's B is multiplied with zeros for the other tokens of a 256-token tile that has one of its own: its values
+    must be finite.  Adapters that no token of a tile names are not read.
+    """
+    if X.dim() != 2 or W.dim() != 2 or X.shape[1] != W.shape[1]:
+        raise RuntimeError("lora_ht_gemm: expected X (N, K) and W (M, K)")
+    N, K = X.shape
+    if out_layout not in ("mn", "nm"):
+        raise RuntimeError("lora_ht_gemm: out_layout must be 'mn' or 'nm'")
+    out_dtype = out_dtype or torch.float32
+    M, adapters, rank, A, B, index, scaling = _check("lora_ht_gemm", X, W, A, B, index, scaling, N, K, out_dtype)
+    X, W = _rows(X), _rows(W)
+    out = _out("lora_ht_gemm", out, (M, N) if out_layout == "mn" else (N, M), out_dtype, X.device)
+    if M == 0 or N == 0:
+        return out
+    lib = _lib.load()
+    mask = None if signs is None else sign_mask(signs, K, X.device)
+    ws = torch.empty(lib.b200ht_lora_gemm_workspace_bytes(M, N, K, rank), dtype=torch.uint8, device=X.device)
+    with _on_device(X.device):
+        rc = lib.b200ht_lora_gemm(X.data_ptr(), W.data_ptr(), out.data_ptr(), A.data_ptr(), B.data_ptr(), index.data_ptr(),
+                                  None if scaling is None else scaling.data_ptr(), M, N, K, adapters, rank, _DT[out_dtype],
+                                  _lib.OUT_MN if out_layout == "mn" else _lib.OUT_NM,
+                                  math.sqrt(1.0 / K) if scale is None else float(scale),
+                                  None if mask is None else mask.data_ptr(), ws.data_ptr(), ws.numel(), _stream_ptr(X.device))
+    _lib.check(rc, "b200ht_lora_gemm")
+    return out
+
+
+def lora_ht_gemv(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Tensor, index: torch.Tensor, *,
+                 scaling: torch.Tensor | None = None, scale: float | None = None, out_dtype: torch.dtype | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """``fused_ht_gemv(W, X)`` plus the adapter of each column: one token of every request of a decoding batch.
+
+    ``W`` is (M, N), ``X`` (N, columns) with the columns fastest (or a vector, one column), the result (M, columns);
+    ``A`` (adapters, rank, N), ``B`` (adapters, M, rank), ``index`` (columns int32 entries) and ``scaling`` as in
+    :func:`lora_ht_gemm`.  The low-rank vectors stay fp32 and Y is rounded once.  Beyond the batch that
+    ``fused_ht_gemv`` serves with one pass over W the call goes through :func:`lora_ht_gemm`.
+    """
+    if X.dim() == 1:
+        X = X[:, None]
+    if X.dim() != 2 or W.dim() != 2 or X.shape[0] != W.shape[1]:
+        raise RuntimeError("lora_ht_gemv: expected W (M, N) and X (N, B)")
+    N, columns = X.shape
+    if columns < 1:
+        raise RuntimeError("lora_ht_gemv: batch must be at least 1, got 0")
+    out_dtype = out_dtype or torch.float32
+    lib = _lib.load()
+    once = lib.b200ht_fused_gemv_max_batch(N, _lib.BF16)   # columns served by one pass over W
+    if columns > _MAX_COLUMNS or (once and columns > once):
+        return lora_ht_gemm(X.t(), W, A, B, index, scaling=scaling, scale=scale, out_dtype=out_dtype, out=out)
+    M, adapters, rank, A, B, index, scaling = _check("lora_ht_gemv", X, W, A, B, index, scaling, columns, N, out_dtype)
+    X, W = _rows(X), _rows(W)
+    out = _out("lora_ht_gemv", out, (M, columns), out_dtype, X.device)
+    if M == 0:
+        return out
+    ws = torch.empty(lib.b200ht_lora_gemv_workspace_bytes(M, columns, rank), dtype=torch.uint8, device=X.device)
+    with _on_device(X.device):
+        rc = lib.b200ht_lora_gemv(W.data_ptr(), X.data_ptr(), out.data_ptr(), A.data_ptr(), B.data_ptr(), index.data_ptr(),
+                                  None if scaling is None else scaling.data_ptr(), M, N, columns, adapters, rank,
+                                  _DT[out_dtype], math.sqrt(1.0 / N) if scale is None else float(scale), ws.data_ptr(),
+                                  ws.numel(), _stream_ptr(X.device))
+    _lib.check(rc, "b200ht_lora_gemv")
+    return out

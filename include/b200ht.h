@@ -277,6 +277,38 @@ int b200ht_norm_rotary_qk_backward(const void *dq_out, const void *dk_out, const
                                    void *stream);
 
 /*
+ * b200ht_fused_gemm (bf16) with the low-rank adapter of each token's request beside the shared projection:
+ *   C[m, t] = sum_k W[m, k] * (scale * H_K (d * x_t))[k]  +  scaling[a] * sum_r B[a][m][r] * sum_k A[a][r][k] * x_t[k]
+ * with a = index[t].  A token whose index lies outside 0 .. adapters - 1 (-1, say) has no adapter.  The adapter sees the
+ * tokens as given: neither the transform nor the signs d apply to it.  No counterpart in the reference.
+ *   A        adapters x rank x K bf16;  B  adapters x M x rank bf16;  both 16-byte aligned
+ *   index    N 32-bit integers, in any order; tokens of one request next to each other cost least (a 256-token tile
+ *            pays rank / K of its contraction for each adapter among its tokens)
+ *   scaling  one float per adapter, or NULL for 1
+ *   signs    as in b200ht_fused_gemm_signed, or NULL
+ * K a power of two, 64 .. 32768; rank a multiple of 8, 8 .. 128 (pad with rows and columns of zeros).  W, X, A, B bf16;
+ * the low-rank vectors are rounded to bf16 once, like H(X), everything else is accumulated in fp32.
+ * An adapter's B takes part in the contraction of every 256-token tile with one of its tokens, against zeros for the
+ * other tokens: infinities or NaN in B reach those tokens too.  Adapters that no token of a tile has are not read.
+ * `workspace`: b200ht_lora_gemm_workspace_bytes(M, N, K, rank) bytes, 256-byte aligned.  Calls that share one must not
+ * run at the same time.
+ */
+size_t b200ht_lora_gemm_workspace_bytes(int M, int N, int K, int rank);
+int b200ht_lora_gemm(const void *X, const void *W, void *C, const void *A, const void *B, const int *index,
+                     const float *scaling, int M, int N, int K, int adapters, int rank, int out_dtype, int out_layout,
+                     float scale, const void *signs, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The same for a decoding batch, in the layouts of b200ht_fused_gemv (bf16): X  N x B with b fastest, Y  M x B with b
+ * fastest, index[b] the adapter of column b, 1 <= B <= 64, N a power of two, 64 .. 32768.  The low-rank vectors stay
+ * fp32; one rounding.  `workspace`: b200ht_lora_gemv_workspace_bytes(M, B, rank) bytes, 256-byte aligned.
+ */
+size_t b200ht_lora_gemv_workspace_bytes(int M, int B, int rank);
+int b200ht_lora_gemv(const void *W, const void *X, void *Y, const void *A, const void *Bm, const int *index,
+                     const float *scaling, int M, int N, int B, int adapters, int rank, int out_dtype, float scale,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Number of kernels this library has launched in the calling process so far (all entry points, all streams).
  * A benchmark reads it before and after a timed region to report its launch count.  No counterpart in the reference.
  */

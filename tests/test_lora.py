@@ -1,0 +1,367 @@
+"""W . H(X) with the adapters of many requests, against the definition in 64 bits.
+
+The base product is tested elsewhere; here the adapters' share is looked at by itself, as the difference between a call
+with fp32 results and the same call without adapters (same transform, same order of the base's sums, so the base cancels
+up to the roundings named below).  With S_r = scaling * sum_k A_rk x_k the share is sum_r B_mr S_r.  Its error:
+
+* S: a sum of K products in fp32, off by at most K units of 2^-24 of the sum of their sizes, however it is ordered; times
+  the scaling, one unit; for the tensor cores rounded to bf16, 2^-8 of its size;
+* B S: rank products (exact in fp32) added to a sum that already holds the base: the tensor cores add 16 products at a
+  time and may cut instead of rounding, so each of the rank / 16 + 1 additions is off by at most 2^-22 of the largest
+  size the sum can have; by fp32 arithmetic (decoding) rank + 2 additions by 2^-23 each;
+* the difference of the two results itself is fp64.
+"""
+import ctypes
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+
+
+def make(N, K, M, R, L, seed=0, spread="runs", device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+
+    def normal(*shape, by=1.0):
+        return (torch.randn(*shape, generator=g) * by).bfloat16().to(device)
+
+    X, W = normal(N, K), normal(M, K, by=K ** -0.5)
+    A, B = normal(L, R, K, by=K ** -0.5), normal(L, M, R, by=R ** -0.5)
+    scaling = (0.25 + torch.rand(L, generator=g)).to(device)
+    if spread == "runs":        # requests of many tokens, one in four without an adapter
+        cuts = torch.sort(torch.randint(0, N + 1, (max(1, min(7, N // 3)),), generator=g)).values
+        of = torch.randint(-1, L, (len(cuts) + 1,), generator=g)
+        index = of[torch.bucketize(torch.arange(N), cuts, right=True)]
+    elif spread == "any":       # every token its own, values outside the range among them
+        index = torch.randint(-2, L + 2, (N,), generator=g)
+    else:
+        index = torch.full((N,), int(spread))
+    return X, W, A, B, index.int().to(device), scaling
+
+
+def share64(X, A, B, index, scaling):
+    """The adapters' share (tokens, M) in 64 bits, the bound of its error that comes from S in units of its factors, and
+    the sum of the sizes of its products."""
+    L = A.shape[0]
+    X, A, B, index = X.double().cpu(), A.double().cpu(), B.double().cpu(), index.cpu().long()
+    sc = torch.ones(L, dtype=torch.float64) if scaling is None else scaling.double().cpu()
+    N, M = X.shape[0], B.shape[1]
+    out, s_unit, size = (torch.zeros(N, M, dtype=torch.float64) for _ in range(3))
+    for a in range(L):
+        rows = (index == a).nonzero()[:, 0]
+        if len(rows):
+            S = X[rows] @ A[a].t() * sc[a]
+            out[rows] = S @ B[a].t()
+            size[rows] = S.abs() @ B[a].abs().t()
+            s_unit[rows] = (X[rows].abs() @ A[a].abs().t() * sc[a].abs()) @ B[a].abs().t()
+    return out, s_unit, size
+
+
+def check_share(got, base, X, A, B, index, scaling, tensor_cores=True):
+    """got, base: fp32 results (tokens, M) with and without adapters."""
+    want, s_unit, size = share64(X, A, B, index, scaling)
+    K, R = X.shape[1], A.shape[1]
+    got, base = got.double().cpu(), base.double().cpu()
+    allowed = (K + 1) * U * s_unit
+    biggest = base.abs() + size * (1 + 2.0 ** -8) + allowed
+    if tensor_cores:
+        allowed = allowed + size * 2.0 ** -8 + (R // 16 + 2) * 2.0 ** -22 * biggest
+    else:
+        allowed = allowed + (R + 2) * 2.0 ** -23 * biggest
+    off = (got - base - want).abs()
+    assert bool((off <= allowed).all()), f"off by {float((off - allowed).max()):.3g} too much"
+    none = (index.cpu() < 0) | (index.cpu() >= A.shape[0])
+    assert torch.equal(got[none], base[none])   # tokens without an adapter: bit for bit the base
+
+
+# ---------------------------------------------------------------------------------------------------- without a GPU
+def test_refusals_of_the_python_entries(pkg):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with pytest.raises(RuntimeError, match="CUDA"):
+        X, W, A, B, index, sc = make(4, 64, 32, 8, 2, device="cpu")
+        pkg.lora_ht_gemm(X, W, A, B, index)
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.bfloat16, device="cuda"):
+            return torch.empty(*shape, dtype=dtype, device=device)
+
+        i32, f32 = torch.int32, torch.float32
+        good = {"X": t(20, 128), "W": t(48, 128), "A": t(3, 16, 128), "B": t(3, 48, 16), "index": t(20, dtype=i32)}
+        bad = [
+            {"X": t(20, 128, dtype=f32)}, {"W": t(48, 128, dtype=f32)}, {"A": t(3, 16, 128, dtype=torch.float16)},
+            {"X": t(20, 64)}, {"X": t(2, 10, 128)}, {"W": t(48, 128, device="cpu")}, {"index": t(20, dtype=i32, device="cpu")},
+            {"A": t(16, 128)}, {"A": t(2, 16, 128)}, {"B": t(3, 47, 16)}, {"B": t(3, 48, 8)}, {"A": t(3, 12, 128), "B": t(3, 48, 12)},
+            {"A": t(3, 136, 128), "B": t(3, 48, 136)}, {"A": t(0, 16, 128), "B": t(0, 48, 16)},
+            {"A": t(3, 0, 128), "B": t(3, 48, 0)}, {"index": t(20, dtype=torch.int64)}, {"index": t(19, dtype=i32)},
+            {"X": t(20, 32), "W": t(48, 32), "A": t(3, 16, 32)}, {"X": t(20, 96), "W": t(48, 96), "A": t(3, 16, 96)},
+            {"scaling": t(3)}, {"scaling": t(4, dtype=f32)}, {"out_dtype": torch.float16}, {"out_layout": "tm"},
+            {"out": t(20, 48, dtype=f32)}, {"out": t(48, 20)},
+        ]
+        for change in bad:
+            with pytest.raises(RuntimeError):
+                pkg.lora_ht_gemm(**{**good, **change})
+        del good["X"]
+        columns = {"X": t(128, 20), **good}
+        for change in ({"X": t(128, 0)}, {"X": t(64, 20)}, {"index": t(3, dtype=i32)}, {"B": t(3, 48, 8)}, {"out": t(20, 48)},
+                       {"W": t(48, 128, dtype=f32)}, {"scaling": t(2, dtype=f32)}):
+            with pytest.raises(RuntimeError):
+                pkg.lora_ht_gemv(**{**columns, **change})
+
+
+def test_c_entries_refuse_before_the_gpu(lib):
+    l = lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) & ~255
+
+    def gemm(X=p, W=p, C=p, A=p, B=p, index=p, scaling=p, M=48, N=20, K=128, L=3, R=16, odt=lib.F32, layout=0, signs=None, ws=p,
+             nws=1 << 30):
+        return l.b200ht_lora_gemm(X, W, C, A, B, index, scaling, M, N, K, L, R, odt, layout, 1.0, signs, ws, nws, None)
+
+    def gemv(X=p, W=p, C=p, A=p, B=p, index=p, scaling=p, M=48, N=20, K=128, L=3, R=16, odt=lib.F32, ws=p, nws=1 << 30):
+        return l.b200ht_lora_gemv(W, X, C, A, B, index, scaling, M, K, N, L, R, odt, 1.0, ws, nws, None)
+
+    for f in (gemm, gemv):
+        assert f(odt=lib.F16) == -3
+        for how in ({"K": 96}, {"K": 32}, {"K": 1 << 16}, {"M": -1}, {"N": -1}, {"L": 0}, {"R": 0}, {"R": 12}, {"R": 136}):
+            assert f(**how) == -2, how
+        for how in ({"X": None}, {"W": None}, {"C": None}, {"A": None}, {"B": None}, {"index": None}):
+            assert f(**how) == -1, how
+        for how in ({"X": p + 2}, {"A": p + 8}, {"B": p + 8}, {"C": p + 4}, {"index": p + 2}, {"scaling": p + 2}, {"ws": p + 128}):
+            assert f(**how) == -4, how
+        assert f(ws=None) == -5 and f(nws=64) == -5
+        assert f(M=0, X=None) == 0
+    assert gemm(layout=2) == -2 and gemm(signs=p + 2) == -4 and gemm(N=0, X=None) == 0
+    assert gemv(N=0) == -2 and gemv(N=65) == -2
+    assert l.b200ht_lora_gemm_workspace_bytes(48, 20, 128, 16) >= 20 * 128 * 2 + 20 * 16 * 2
+    assert l.b200ht_lora_gemm_workspace_bytes(48, 0, 128, 16) == 0
+    assert l.b200ht_lora_gemv_workspace_bytes(48, 20, 16) >= (48 * 20 + 20 * 16) * 4
+
+
+# --------------------------------------------------------------------------------------------------------- on the GPU
+SHAPES = [
+    # tokens, K, M, rank, adapters
+    (1, 64, 8, 8, 1), (1, 1024, 300, 16, 4), (3, 256, 130, 64, 5), (17, 512, 64, 24, 3), (64, 1024, 96, 128, 2),
+    (65, 128, 200, 8, 40), (127, 512, 77, 32, 3), (129, 256, 256, 72, 6), (255, 64, 129, 16, 100), (256, 1024, 384, 64, 4),
+    (257, 512, 1, 40, 2), (300, 2048, 130, 120, 9), (1000, 256, 520, 16, 7), (1537, 512, 250, 56, 30), (700, 4096, 64, 128, 3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("spread", ["runs", "any"])
+@pytest.mark.parametrize("layout", ["mn", "nm"])
+def test_prompts(pkg, shape, spread, layout):
+    N, K, M, R, L = shape
+    X, W, A, B, index, scaling = make(N, K, M, R, L, seed=N, spread=spread)
+    base = pkg.fused_ht_gemm(X, W, out_layout=layout)
+    got = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout=layout)
+    half = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout=layout, out_dtype=torch.bfloat16)
+    assert pkg.device_status() == 0
+    assert torch.equal(half, got.bfloat16())   # the same sums, rounded once
+    if layout == "mn":
+        base, got = base.t(), got.t()
+    check_share(got, base, X, A, B, index, scaling)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("index", ["-1", "0", "2", "7"])
+def test_one_adapter_or_none_for_all(pkg, index):
+    X, W, A, B, index, _ = make(400, 512, 200, 16, 3, spread=index)
+    base = pkg.fused_ht_gemm(X, W, out_layout="nm")
+    check_share(pkg.lora_ht_gemm(X, W, A, B, index, out_layout="nm"), base, X, A, B, index, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,M,L", [(2560, 64, 4096, 3), (2500, 64, 4090, 200), (1100, 32768, 130, 4), (20000, 2048, 40, 5)])
+def test_split_launches_and_chunks(pkg, N, K, M, L):
+    """The contraction in two launches (160 tiles of 256 rows on 148 SMs), and tokens in chunks that keep their transform in
+    L2: tables, low-rank vectors and rows of B have to move along."""
+    X, W, A, B, index, scaling = make(N, K, M, 16, L, seed=5)
+    base = pkg.fused_ht_gemm(X, W, out_layout="nm")
+    got = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout="nm")
+    assert pkg.device_status() == 0
+    check_share(got, base, X, A, B, index, scaling)
+
+
+@pytest.mark.gpu
+def test_signs_and_scale_belong_to_the_transform(pkg):
+    X, W, A, B, index, scaling = make(270, 512, 140, 32, 4, seed=6)
+    signs = torch.randint(0, 2, (512,), generator=torch.Generator().manual_seed(1)).cuda() * 2 - 1
+    base = pkg.fused_ht_gemm(X, W, signs=signs, scale=0.5, out_layout="nm")
+    got = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, signs=signs, scale=0.5, out_layout="nm")
+    check_share(got, base, X, A, B, index, scaling)
+
+
+COLUMNS = [
+    # columns, N, M, rank, adapters
+    (1, 64, 8, 8, 1), (1, 4096, 1000, 64, 3), (1, 8192, 333, 128, 2), (2, 256, 31, 16, 5), (5, 1024, 130, 24, 2), (16, 4096, 97, 16, 20),
+    (13, 512, 65, 72, 4), (8, 8192, 40, 32, 3), (24, 2048, 50, 8, 9), (32, 1024, 70, 120, 5), (64, 128, 33, 64, 6), (3, 32768, 20, 16, 2),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", COLUMNS, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("spread", ["any", "0", "-1"])
+def test_decoding(pkg, shape, spread):
+    columns, N, M, R, L = shape
+    X, W, A, B, index, scaling = make(columns, N, M, R, L, seed=columns, spread=spread)
+    Xc = X.t().contiguous()
+    base = pkg.fused_ht_gemv(W, Xc)
+    got = pkg.lora_ht_gemv(W, Xc, A, B, index, scaling=scaling)
+    half = pkg.lora_ht_gemv(W, Xc, A, B, index, scaling=scaling, out_dtype=torch.bfloat16)
+    assert pkg.device_status() == 0
+    assert torch.equal(half, got.bfloat16())
+    check_share(got.t(), base.t(), X, A, B, index, scaling, tensor_cores=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("columns", [17, 40, 64, 100])
+def test_decoding_beyond_one_pass_over_the_weight(pkg, columns):
+    X, W, A, B, index, scaling = make(columns, 4096, 100, 16, 6, seed=8, spread="any")
+    got = pkg.lora_ht_gemv(W, X.t().contiguous(), A, B, index, scaling=scaling)
+    assert got.shape == (100, columns)
+    check_share(got.t(), pkg.fused_ht_gemm(X, W, out_layout="nm"), X, A, B, index, scaling)
+
+
+@pytest.mark.gpu
+def test_a_vector_is_one_column(pkg):
+    X, W, A, B, index, scaling = make(1, 1024, 50, 8, 2, spread="1")
+    assert torch.equal(pkg.lora_ht_gemv(W, X[0], A, B, index), pkg.lora_ht_gemv(W, X.t().contiguous(), A, B, index))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [40, 600])
+def test_what_a_token_does_not_own_does_not_reach_it(pkg, N):
+    """NaN in the memory of adapters that no token names, and in one token's values, stay where they are."""
+    X, W, A, B, index, scaling = make(N, 256, 140, 16, 6, seed=9, spread="any")
+    index[index == 3] = 2
+    clean = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout="nm")
+    A2, B2, sc2, X2 = A.clone(), B.clone(), scaling.clone(), X.clone()
+    A2[3], B2[3], sc2[3] = float("nan"), float("inf"), float("nan")
+    assert torch.equal(pkg.lora_ht_gemm(X, W, A2, B2, index, scaling=sc2, out_layout="nm"), clean)
+    X2[17, 5] = float("nan")
+    X2[33, 6] = float("inf")
+    got = pkg.lora_ht_gemm(X2, W, A2, B2, index, scaling=sc2, out_layout="nm")
+    others = [t for t in range(N) if t not in (17, 33)]
+    assert torch.equal(got[others], clean[others]) and torch.isnan(got[17]).all() and not torch.isfinite(got[33]).any()
+    Xc = X[:16].t().contiguous()
+    clean = pkg.lora_ht_gemv(W, Xc, A, B, index[:16], scaling=scaling)
+    assert torch.equal(pkg.lora_ht_gemv(W, Xc, A2, B2, index[:16], scaling=sc2), clean)
+
+
+@pytest.mark.gpu
+def test_views_and_outputs_in_hand(pkg):
+    """Strided and oddly aligned inputs are taken (copied where need be); `out` is written in place."""
+    X, W, A, B, index, scaling = make(90, 256, 64, 16, 3, seed=10)
+    want = pkg.lora_ht_gemm(X, W, A, B, index, out_layout="nm")
+    raw = torch.empty(A.numel() + 1, dtype=A.dtype, device="cuda")
+    odd = raw[1:].view(A.shape).copy_(A)
+    wide = torch.zeros(90, 512, dtype=X.dtype, device="cuda")
+    wide[:, 128:384] = X
+    every = torch.stack([index, index], 1)[:, 0]
+    out = torch.empty(90, 64, device="cuda")
+    got = pkg.lora_ht_gemm(wide[:, 128:384], W.t().contiguous().t(), odd, B.transpose(1, 2).contiguous().transpose(1, 2), every,
+                           out_layout="nm", out=out)
+    assert got is out and torch.equal(got, want)
+    assert pkg.lora_ht_gemm(X[:0], W, A, B, index[:0], out_layout="nm").shape == (0, 64)
+    with pytest.raises(RuntimeError, match="out has"):
+        pkg.lora_ht_gemm(X, W, A, B, index, out_layout="nm", out=torch.empty(64, 90, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_graphs_streams_and_repeats(pkg):
+    """Captured twice and replayed side by side on two streams; the same bits on every call."""
+    X, W, A, B, index, scaling = make(513, 1024, 320, 32, 12, seed=11, spread="any")
+    Xc = X[:16].t().contiguous()
+
+    def call():
+        return (pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout="nm", out_dtype=torch.bfloat16),
+                pkg.lora_ht_gemv(W, Xc, A, B, index[:16], scaling=scaling))
+
+    want = call()
+    for _ in range(3):
+        for a, b in zip(call(), want):
+            assert torch.equal(a, b)
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(call())
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for out in outs:
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+    assert pkg.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_writes_stay_in_the_result_and_the_workspace(pkg, lib):
+    l = lib.load()
+    for N, K, M, R, L, layout in ((3, 64, 33, 8, 2, 1), (300, 256, 130, 24, 5, 0), (129, 512, 257, 128, 40, 1)):
+        X, W, A, B, index, scaling = make(N, K, M, R, L, seed=12, spread="any")
+        n = l.b200ht_lora_gemm_workspace_bytes(M, N, K, R)
+        guard = 4096
+        ws = torch.full((n + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda")
+        C = torch.full((guard + M * N * 2 + (-M * N * 2) % 256 + guard,), 0xA5, dtype=torch.uint8, device="cuda")
+        rc = l.b200ht_lora_gemm(X.data_ptr(), W.data_ptr(), C.data_ptr() + guard, A.data_ptr(), B.data_ptr(), index.data_ptr(),
+                                scaling.data_ptr(), M, N, K, L, R, lib.BF16, layout, K ** -0.5, None, ws.data_ptr() + guard, n,
+                                torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, lib.error_string(rc)
+        want = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout="nm" if layout else "mn", out_dtype=torch.bfloat16)
+        assert torch.equal(C[guard:guard + M * N * 2].view(torch.bfloat16), want.view(-1))
+        for z in (ws[:guard], ws[guard + n:], C[:guard], C[guard + M * N * 2:]):
+            assert bool((z == 0xA5).all())
+        if N <= 64:
+            n = l.b200ht_lora_gemv_workspace_bytes(M, N, R)
+            ws = torch.full((n + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda")
+            C.fill_(0xA5)
+            Xc = X.t().contiguous()
+            rc = l.b200ht_lora_gemv(W.data_ptr(), Xc.data_ptr(), C.data_ptr() + guard, A.data_ptr(), B.data_ptr(), index.data_ptr(),
+                                    None, M, K, N, L, R, lib.BF16, K ** -0.5, ws.data_ptr() + guard, n,
+                                    torch.cuda.current_stream().cuda_stream)
+            assert rc == 0, lib.error_string(rc)
+            want = pkg.lora_ht_gemv(W, Xc, A, B, index, out_dtype=torch.bfloat16)
+            assert torch.equal(C[guard:guard + M * N * 2].view(torch.bfloat16), want.view(-1))
+            for z in (ws[:guard], ws[guard + n:], C[:guard], C[guard + M * N * 2:]):
+                assert bool((z == 0xA5).all())
+
+
+@pytest.mark.gpu
+def test_projection_with_adapters_then_norm_and_rotation(pkg):
+    """The operators as a layer runs them: one product for queries, keys and values of a prompt, views of it through norm and
+    rotation, and the next token of the same requests by the decoding forms, which has to agree with the prompt's."""
+    T, K, D, hq, hk, L, R = 70, 1024, 64, 6, 2, 3, 16
+    M = (hq + 2 * hk) * D
+    X, W, A, B, index, scaling = make(T, K, M, R, L, seed=13)
+    g = torch.Generator().manual_seed(14)
+    qw, kw = ((1 + 0.1 * torch.randn(D, generator=g)).bfloat16().cuda() for _ in range(2))
+    pos = torch.arange(T, device="cuda") + 5000
+    inv = (1e4 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))).float().cuda()
+    qkv = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout="nm", out_dtype=torch.bfloat16).view(T, -1, D)
+    q, k = pkg.norm_rotary_qk(qkv[:, :hq], qkv[:, hq:hq + hk], qw, kw, pos, inv, hadamard=True)
+    # the heads' kernel against the definition, on the projection as it came out
+    from tests.test_heads import assert_close, forward64
+    assert_close(q, forward64(qkv[:, :hq], qw, 1e-6, pos, inv, hadamard=True))
+    assert_close(k, forward64(qkv[:, hq:hq + hk], kw, 1e-6, pos, inv, hadamard=True))
+    # the last eight tokens again, one call each for all of them
+    last = slice(T - 8, T)
+    one = pkg.lora_ht_gemv(W, X[last].t().contiguous(), A, B, index[last], scaling=scaling, out_dtype=torch.bfloat16)
+    one = one.t().contiguous().view(8, -1, D)
+    # Both forms round H(X) to bf16 (at most four times on the way, 2^-8 of the row's norm each), S in one of them, and the
+    # result: 2^-8 of |W_m| |x| |H(x)| at most each; the norm and rotation then keep distances relative to the row.
+    x64 = X[last].double()
+    room = (4 + 4 + 2) * 2.0 ** -8 * (W.double().norm(dim=1)[None] * x64.norm(dim=1)[:, None]).cpu()
+    want, s_unit, size = share64(X[last], A, B, index[last], scaling)
+    room = room + size * 2.0 ** -7 + qkv[last].double().abs().view(8, M).cpu() * 2.0 ** -7
+    assert bool(((one.double() - qkv[last].double()).abs().view(8, M).cpu() <= room).all())
+    q1, k1 = pkg.norm_rotary_qk(one[:, :hq], one[:, hq:hq + hk], qw, kw, pos[last], inv, hadamard=True)
+    assert_close(q1, forward64(one[:, :hq], qw, 1e-6, pos[last], inv, hadamard=True))
+    assert k1.shape == (8, hk, D)
