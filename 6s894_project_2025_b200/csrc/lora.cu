@@ -167,6 +167,197 @@ lora_expand_kernel(const float *base, const __nv_bfloat16 *B, const float *S, co
 }
 
 // ---------------------------------------------------------------------------
+// S of many tokens, on the tensor cores: 128 tokens (the M of the instruction) against the adapters among them (N: `width`
+// columns an adapter, its rank to a multiple of 16), K split over the CTAs of a cluster.  Each token keeps the columns of
+// its own adapter; the tile's list of adapters is walked in passes of `per_pass` (128 columns of TMEM).  With prompts a
+// tile has one or two adapters and X is read once; bound then: the bytes of X.
+//
+// Warp 0 copies by TMA (X 128 x 64 and `width` x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the
+// MMAs, warps 2..5 bring the accumulator (one token a lane) into shared memory, over the stages that have been used up.
+// The CTAs of the cluster then add the partial sums of 128 / cluster tokens each through distributed shared memory, in
+// the order of the ranks, and write them with one rounding: no atomics, no partial sums in memory.
+// ---------------------------------------------------------------------------
+constexpr int kShrinkTokens = 128, kShrinkStages = 3, kShrinkThreads = 192, kShrinkColumns = 128;
+constexpr int kShrinkXBytes = kShrinkTokens * 128, kShrinkABytes = kShrinkColumns * 128;
+constexpr int kShrinkStageBytes = kShrinkXBytes + kShrinkABytes;
+constexpr int kShrinkSmem = kShrinkStages * kShrinkStageBytes + 1024 + 128;
+static_assert(kShrinkTokens * (kLoraMaxRank + 1) * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
+
+__device__ __forceinline__ void cluster_sync_all()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ float cluster_load(uint32_t local, int rank)   // the float at `local` in the shared memory of CTA `rank`
+{
+    float v;
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__global__ void __launch_bounds__(kShrinkThreads, 2)
+lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const int *tiles,
+                        const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int adapters, int rank, int width,
+                        int per_pass, int kblocks, int split, int *status)
+{
+    extern __shared__ unsigned char smem_dyn[];
+    __shared__ int ids[kShrinkTokens], list[kShrinkTokens];   // adapter of each token; the adapters of the tile
+    __shared__ float factor[kShrinkTokens];                   // scaling of each token's adapter
+    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+    unsigned char *gen = smem_dyn + (base - smem_u32(smem_dyn));
+    const uint32_t bars = base + kShrinkStages * kShrinkStageBytes;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (kShrinkStages + s); };
+    const uint32_t done_bar = bars + 16u * kShrinkStages;
+    uint32_t *tmem_slot = (uint32_t *)(gen + kShrinkStages * kShrinkStageBytes + 16 * kShrinkStages + 8);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int part = blockIdx.x % split, tile = blockIdx.x / split;   // rank in the cluster, 128-token tile
+    const int t0 = tile * kShrinkTokens;
+
+    if (tid == 0) {
+        for (int s = 0; s < kShrinkStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmX);
+        tma_prefetch_desc(&tmA);
+    }
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), kShrinkColumns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();   // not before this CTA has its TMEM: the contraction behind takes all of it
+    pdl_wait();
+
+    const int *table = tiles + (size_t)(tile >> 1) * kLoraTileInts + kLoraHalfOffset + (tile & 1) * kLoraHalfInts;
+    const int count = __ldcg(table);
+    if (tid < kShrinkTokens) {
+        const int id = t0 + tid < tokens ? __ldcg(index + t0 + tid) : -1;
+        ids[tid] = id;
+        factor[tid] = scaling && (unsigned)id < (unsigned)adapters ? scaling[id] : 1.f;
+        if (tid < count) list[tid] = __ldcg(table + 1 + tid);
+    }
+    __syncthreads();
+    const int kb0 = kblocks / split * part, kb1 = kb0 + kblocks / split;
+    float *partial = (float *)gen;                  // [128][rank + 1], over the stages
+    const int pitch = rank + 1;
+    const int rows = kShrinkTokens / split, row0 = part * rows;   // tokens whose sums this CTA writes
+    if (blockIdx.y == 0)                            // tokens without an adapter
+        for (int i = tid; i < rows * (rank / 8); i += kShrinkThreads) {
+            const int t = t0 + row0 + i / (rank / 8);
+            if (t < tokens && (unsigned)ids[t - t0] >= (unsigned)adapters)
+                *(uint4 *)(S + (size_t)t * rank + i % (rank / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+        }
+
+    uint32_t it = 0, passes = 0;
+    bool ok = true;   // once a wait has run out this CTA copies and multiplies no more, but keeps step with its cluster
+    for (int first = blockIdx.y * per_pass; first < count; first += gridDim.y * per_pass, ++passes) {
+        const int n = count - first < per_pass ? count - first : per_pass;
+        if (!ok) {
+        } else if (warp == 0 && lane == 0) {
+            uint32_t i2 = it;
+            for (int kb = kb0; kb < kb1 && ok; ++kb, ++i2) {
+                const int s = i2 % kShrinkStages;
+                if (!mbar_wait(empty_bar(s), ((i2 / kShrinkStages) & 1u) ^ 1u, abort_flag, status)) { ok = false; break; }
+                mbar_expect_tx(full_bar(s), (uint32_t)(kShrinkXBytes + n * width * 128));
+                const uint32_t sa = base + s * kShrinkStageBytes;
+                tma_load_3d(sa, &tmX, kb * 64, t0, 0, full_bar(s));
+                for (int a = 0; a < n; ++a)
+                    tma_load_3d(sa + kShrinkXBytes + a * width * 128, &tmA, kb * 64, 0, list[first + a], full_bar(s));
+            }
+            if (!ok) {   // copies on their way still land in this CTA's shared memory: give them time
+                const uint32_t pending = i2 < (uint32_t)kShrinkStages ? i2 : (uint32_t)kShrinkStages;
+                for (uint32_t j = 1; j <= pending; ++j) {
+                    const uint64_t ns = global_ns();
+                    while (!mbar_test(full_bar((i2 - j) % kShrinkStages), ((i2 - j) / kShrinkStages) & 1u) && global_ns() - ns < 100000000ull) {}
+                }
+            }
+        } else if (warp == 1 && lane == 0) {
+            const uint32_t idesc = umma_idesc_bf16(kShrinkTokens, width);
+            uint32_t i2 = it;
+            for (int kb = kb0; kb < kb1; ++kb, ++i2) {
+                const int s = i2 % kShrinkStages;
+                if (!mbar_wait(full_bar(s), (i2 / kShrinkStages) & 1u, abort_flag, status)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t sa = base + s * kShrinkStageBytes;
+                const uint64_t xdesc = umma_desc_k_sw128(sa);
+                for (int a = 0; a < n; ++a) {
+                    const uint64_t adesc = umma_desc_k_sw128(sa + kShrinkXBytes + a * width * 128);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_bf16_ss(tmem + a * width, xdesc + 2 * k, adesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
+                }
+                umma_commit(empty_bar(s));
+            }
+            if (ok) umma_commit(done_bar);
+        }
+        __syncwarp();
+        it += (uint32_t)(kb1 - kb0);
+        // all MMAs of the pass done: the accumulator is complete and the stages are free
+        ok = __syncthreads_and(ok && mbar_wait(done_bar, passes & 1u, abort_flag, status));
+        if (ok && warp >= 2) {
+            tc_fence_after();
+            const int q = warp & 3, row = q * 32 + lane;
+            const int id = ids[row];
+            for (int a = 0; a < n; ++a) {
+                const bool mine = id == list[first + a];
+                if (!__any_sync(0xffffffffu, mine)) continue;
+                for (int c = 0; c < rank; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + a * width + c, v);
+                    tmem_ld_wait();
+                    if (mine)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (c + i < rank) partial[row * pitch + c + i] = __uint_as_float(v[i]);
+                }
+            }
+            tc_fence_before();
+        }
+        cluster_sync_all();
+        for (int i = tid; i < rows * rank && ok; i += kShrinkThreads) {
+            const int row = row0 + i / rank, r = i % rank, id = ids[row];
+            bool mine = false;
+            for (int a = 0; a < n; ++a) mine |= id == list[first + a];
+            if (!mine) continue;
+            const uint32_t at = base + (uint32_t)((row * pitch + r) * 4);
+            float v[8], sum = 0.f;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) v[p] = p < split ? cluster_load(at, p) : 0.f;
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < split) sum += v[p];
+            S[(size_t)(t0 + row) * rank + r] = __float2bfloat16_rn(sum * factor[row]);
+        }
+        fence_proxy_async();   // the next pass' copies overwrite what was read here
+        cluster_sync_all();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kShrinkColumns);
+    }
+}
+
+// ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 template <typename OUT>
@@ -185,6 +376,46 @@ static int launch_shrink_rows(const void *X, const void *A, const int *index, co
     if (rc) return rc;
     return launch_pdl(lora_shrink_rows_kernel<false, OUT>, grid, dim3(256), smem, st, (const __nv_bfloat16 *)X,
                       (const __nv_bfloat16 *)A, index, scaling, S, tokens, K, adapters, rank, rows);
+}
+
+// Tokens from which the tile kernel serves a prompt (see launch_shrink_tiles).
+constexpr int kShrinkTileMin = 65;
+
+static int launch_shrink_tiles(const void *X, const void *A, const int *index, const float *scaling, const int *tiles,
+                               __nv_bfloat16 *S, int tokens, int K, int adapters, int rank, cudaStream_t st)
+{
+    const int width = (rank + 15) & ~15, per_pass = kShrinkColumns / width;
+    CUtensorMap tx, ta;
+    int rc = encode_tmap_bf16_stack(&tx, X, 1, (uint64_t)tokens, (uint64_t)K, kShrinkTokens);
+    if (rc) return rc;
+    rc = encode_tmap_bf16_stack(&ta, A, (uint64_t)adapters, (uint64_t)rank, (uint64_t)K, (uint32_t)width);
+    if (rc) return rc;
+    rc = ensure_dyn_smem((const void *)lora_shrink_tile_kernel, kShrinkSmem);
+    if (rc) return rc;
+    // K over a cluster of up to eight CTAs while all of them find room at once (two an SM), then the passes over the
+    // adapters of a tile over blockIdx.y the same way
+    const int ntiles = (tokens + kShrinkTokens - 1) / kShrinkTokens, room = 2 * sm_count();
+    int split = 1;
+    while (split < 8 && split * 2 <= K / 64 && ntiles * split * 2 <= room) split *= 2;
+    const int most = adapters < kShrinkTokens ? adapters : kShrinkTokens, passes = (most + per_pass - 1) / per_pass;
+    int ways = room / (ntiles * split);
+    ways = ways < 1 ? 1 : (ways > passes ? passes : ways);
+    note_launch();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ntiles * split), (unsigned)ways);
+    cfg.blockDim = dim3(kShrinkThreads);
+    cfg.dynamicSmemBytes = kShrinkSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, lora_shrink_tile_kernel, tx, ta, tiles, index, scaling, S, tokens, adapters, rank, width,
+                                   per_pass, K / 64, split, status_word_ptr());
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -232,7 +463,8 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     const unsigned ntiles = (unsigned)((N + 255L) / 256);
     rc = launch_pdl(lora_plan_kernel, dim3(ntiles), dim3(256), 0, st, index, N, adapters, tiles);
     if (rc) return rc;
-    rc = launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, true, st);
+    rc = N >= kShrinkTileMin ? launch_shrink_tiles(X, A, index, scaling, tiles, S, N, K, adapters, rank, st)
+                             : launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, true, st);
     if (rc) return rc;
     const LoraGemm lora{B, S, tiles, index, adapters, M, rank, 0};
     return fused_gemm_bf16_lora(X, W, C, M, N, K, out_dtype, out_layout, scale, signs, workspace, st, lora);
