@@ -20,7 +20,8 @@
 // With adapters (ADAPT, b200ht_lora_gemm) the K loop of a tile is followed by one more stretch per adapter among the
 // tile's 256 tokens: its B matrix (128 * MT rows x rank) against the tokens' low-rank vectors S (256 x rank), into the
 // same accumulator, so the adapters cost rank / K of the contraction, no pass over C, and no second rounding.  The
-// tokens of other adapters are taken out of S in shared memory, by the MMA warp between the copy and the instructions.
+// instructions cover the groups of 16 tokens that have a token of the adapter; the tokens of other adapters in these
+// groups are zeroed in shared memory by the MMA warp between the copy and the instructions.
 #include <cstdlib>
 #include <mutex>
 
@@ -146,24 +147,42 @@ struct AdaptArgs<true> {
     CUtensorMap tmS;     // [token][rank]
     const int *tiles;    // kLoraTileInts a 256-token tile: number of its adapters, their numbers, ...
     const int *index;    // adapter of each token
-    int rank;
+    int adapters, rank;
     int row;             // row of B of this launch's first row of C
 };
 
-// Zeroes the rows (128 bytes each) of the 256 x 64 tile at `tile` whose token does not belong to `adapter`; `ids`:
-// adapters of tokens lane, lane + 32, ...  One warp, four rows an instruction.
-__device__ __forceinline__ void tc_mask_rows(uint32_t tile, const int (&ids)[TC_BN / 32], int adapter, int lane)
+// Groups of 16 tokens (bit g: tokens 16 g .. 16 g + 15 of the 256 x 64 tile at `tile`) that have a token of `adapter`.
+// In these groups the rows (128 bytes each) of tokens with another adapter are set to zero; those of tokens without one
+// are zero already.  `ids`: adapters of tokens lane, lane + 32, ... (negative: none).  One warp.
+__device__ __forceinline__ uint32_t tc_adapter_groups(uint32_t tile, const int (&ids)[TC_BN / 32], int adapter, int lane)
 {
+    uint32_t groups = 0, zeroed = 0;
 #pragma unroll
-    for (int i = 0; i < TC_BN / 32; ++i)
+    for (int i = 0; i < TC_BN / 32; ++i) {
+        const uint32_t own = __ballot_sync(0xffffffffu, ids[i] == adapter);
+        const uint32_t other = __ballot_sync(0xffffffffu, ids[i] >= 0 && ids[i] != adapter);
 #pragma unroll
-        for (int r = 0; r < 32; r += 4) {
-            const int row = r + (lane >> 3);
-            if (__shfl_sync(0xffffffffu, ids[i], row) != adapter)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(tile + (uint32_t)((i * 32 + row) * 128 + (lane & 7) * 16)),
-                             "r"(0)
-                             : "memory");
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t bits = 0xffffu << (16 * h);
+            if (!(own & bits)) continue;
+            groups |= 1u << (2 * i + h);
+            if (!(other & bits)) continue;
+            zeroed = 1;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {   // four rows an instruction
+                const int row = 16 * h + r + (lane >> 3);
+                if ((other >> row) & 1u)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(tile + (uint32_t)((i * 32 + row) * 128 + (lane & 7) * 16)),
+                                 "r"(0)
+                                 : "memory");
+            }
         }
+    }
+    if (zeroed) {
+        fence_proxy_async();
+        __syncwarp();
+    }
+    return groups;
 }
 
 template <int OUT_DT, int LAYOUT, int MT, bool ADAPT>
@@ -237,6 +256,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 int mb, nb;
                 tc_tile_coord(tile, mt, nt, ord, mb, nb);
                 const int m0 = mb * Cfg::BM, n0 = nb * TC_BN;
+                int count = 0, queue[4];      // number of adapters, the next four: asked for ahead of the K loop
+                if constexpr (ADAPT) {
+                    const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
+                    count = __ldcg(mine);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) queue[i] = __ldcg(mine + 1 + i);
+                }
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
                     const int s = it % STAGES;
                     const uint32_t ph = (it / STAGES) & 1u;
@@ -248,9 +274,10 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 }
                 if constexpr (ADAPT) {
                     const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
-                    const int count = __ldcg(mine);
                     for (int i = 0; i < count && ok; ++i) {
-                        const int adapter = __ldcg(mine + 1 + i);
+                        const int adapter = queue[0];
+                        queue[0] = queue[1], queue[1] = queue[2], queue[2] = queue[3];
+                        if (i + 4 < count) queue[3] = __ldcg(mine + 5 + i);
                         for (int r = 0; r < adapt.rank; r += TC_BK, ++it) {
                             const int s = it % STAGES;
                             const uint32_t ph = (it / STAGES) & 1u;
@@ -284,6 +311,19 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 const int acc = tcount % NACC;
                 const uint32_t aph = (tcount / NACC) & 1u;
                 const uint32_t d_tmem = tmem_base + acc * TC_BN;   // MT == 2: halves at columns 0 and 256
+                int count = 0, ids[TC_BN / 32], list[TC_BN / 32];  // asked for ahead of the K loop: used behind it
+                if constexpr (ADAPT) {
+                    int mb, nb;
+                    tc_tile_coord(tile, mt, nt, ord, mb, nb);
+                    const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
+                    count = __ldcg(mine);
+#pragma unroll
+                    for (int i = 0; i < TC_BN / 32; ++i) {
+                        const int n = nb * TC_BN + i * 32 + lane;
+                        ids[i] = n < N ? __ldcg(adapt.index + n) : -1;
+                        list[i] = __ldcg(mine + 1 + i * 32 + lane);
+                    }
+                }
                 if (lane == 0) {
                     ok = mbar_wait(tempty_bar(acc), aph ^ 1u, abort_flag, status);
                     tc_fence_after();
@@ -307,39 +347,35 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 if constexpr (ADAPT) {
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     it = __shfl_sync(0xffffffffu, it, 0);
-                    int mb, nb;
-                    tc_tile_coord(tile, mt, nt, ord, mb, nb);
-                    const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
-                    const int count = __ldcg(mine);
-                    int ids[TC_BN / 32];
-                    if (count > 1)
 #pragma unroll
-                        for (int i = 0; i < TC_BN / 32; ++i) {
-                            const int n = nb * TC_BN + i * 32 + lane;
-                            ids[i] = n < N ? __ldcg(adapt.index + n) : -1;
-                        }
+                    for (int i = 0; i < TC_BN / 32; ++i)
+                        if (ids[i] >= adapt.adapters) ids[i] = -1;
                     for (int i = 0; i < count && ok; ++i) {
-                        const int adapter = __ldcg(mine + 1 + i);
+                        int entry = list[0];
+#pragma unroll
+                        for (int j = 1; j < TC_BN / 32; ++j) entry = i >> 5 == j ? list[j] : entry;
+                        const int adapter = __shfl_sync(0xffffffffu, entry, i & 31);
                         for (int r = 0; r < adapt.rank; r += TC_BK, ++it) {
                             const int s = it % STAGES;
                             const uint32_t ph = (it / STAGES) & 1u;
                             ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, abort_flag, status));
                             if (!ok) break;
                             const uint32_t sa = base + s * STAGE_BYTES;
-                            if (count > 1) {   // tokens without an adapter have S = 0 as it is
-                                tc_mask_rows(sa + Cfg::A_BYTES, ids, adapter, lane);
-                                fence_proxy_async();
-                                __syncwarp();
-                            }
+                            uint32_t groups = tc_adapter_groups(sa + Cfg::A_BYTES, ids, adapter, lane);
                             if (lane == 0) {
                                 tc_fence_after();
-                                const uint64_t bdesc = umma_desc_k_sw128(sa + Cfg::A_BYTES);
                                 const int ksteps = adapt.rank - r >= TC_BK ? TC_BK / 16 : (adapt.rank - r + 15) / 16;
+                                while (groups) {   // one stretch of neighbouring groups after the other
+                                    const int g0 = __ffs(groups) - 1, n = __ffs(~(groups >> g0)) - 1;
+                                    groups &= ~(((1u << n) - 1) << g0);
+                                    const uint64_t bdesc = umma_desc_k_sw128(sa + Cfg::A_BYTES + g0 * 2048);
+                                    const uint32_t part = umma_idesc_bf16(128, 16 * n);
 #pragma unroll
-                                for (int h = 0; h < MT; ++h) {
-                                    const uint64_t adesc = umma_desc_k_sw128(sa + h * 16384);
-                                    for (int k = 0; k < ksteps; ++k)
-                                        umma_bf16_ss(d_tmem + h * TC_BN, adesc + 2 * k, bdesc + 2 * k, idesc, 1u);
+                                    for (int h = 0; h < MT; ++h) {
+                                        const uint64_t adesc = umma_desc_k_sw128(sa + h * 16384);
+                                        for (int k = 0; k < ksteps; ++k)
+                                            umma_bf16_ss(d_tmem + h * TC_BN + 16 * g0, adesc + 2 * k, bdesc + 2 * k, part, 1u);
+                                    }
                                 }
                                 umma_commit(empty_bar(s));
                             }
@@ -689,6 +725,7 @@ static int launch_tc_mt(const void *Y, const void *W, void *C, int M, int N, int
         if (rc) return rc;
         ad.tiles = lora->tiles;
         ad.index = lora->index;
+        ad.adapters = lora->adapters;
         ad.rank = lora->rank;
         ad.row = lora->row;
         rc = ensure_dyn_smem((const void *)gemm_tc_kernel<OUT_DT, LAYOUT, MT, true>, Cfg::SMEM_BYTES);

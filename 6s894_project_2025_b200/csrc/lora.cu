@@ -22,11 +22,12 @@ int fused_gemm_bf16_lora(const void *X, const void *W, void *C, int M, int N, in
 
 // ---------------------------------------------------------------------------
 // Which adapters occur in each tile of tokens.  A token whose adapter no earlier token of the tile has opens its entry
-// in the list; the search goes backwards, so that a token next to one of its own request stops at once.
+// in the list.  Earlier tokens of its warp are found by a match; only a warp's first token of an adapter looks through
+// the warps before, four tokens a load.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int tokens, int adapters, int *tiles)
 {
-    __shared__ int ids[256];
+    __shared__ __align__(16) int ids[256];
     __shared__ int opened[2][8];
     pdl_launch_dependents();
     pdl_wait();
@@ -35,13 +36,22 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
     int id = t < tokens ? index[t] : -1;
     if ((unsigned)id >= (unsigned)adapters) id = -1;
     ids[tid] = id;
+    const unsigned alike = __match_any_sync(0xffffffffu, id);   // by all lanes: not behind a condition
+    const bool leads = id >= 0 && (alike & ((1u << lane) - 1)) == 0;
     __syncthreads();
-    bool first = id >= 0, first_half = first;
-    for (int j = tid - 1; j >= 0 && first; --j)
-        if (ids[j] == id) {
-            first = false;
-            if (j >= (tid & 128)) first_half = false;
+    bool before = false, before_half = false;   // an earlier warp has the adapter: of the tile, of its half
+    if (leads) {
+        const int4 *four = (const int4 *)ids;
+        const int half0 = (warp & 4) * 8;
+#pragma unroll 8
+        for (int j = 0; j < warp * 8; ++j) {
+            const int4 v = four[j];
+            const bool hit = v.x == id || v.y == id || v.z == id || v.w == id;
+            before |= hit;
+            before_half |= hit && j >= half0;
         }
+    }
+    const bool first = leads && !before, first_half = leads && !before_half;
     const unsigned b = __ballot_sync(0xffffffffu, first), bh = __ballot_sync(0xffffffffu, first_half);
     if (lane == 0) {
         opened[0][warp] = __popc(b);
@@ -167,18 +177,19 @@ lora_expand_kernel(const float *base, const __nv_bfloat16 *B, const float *S, co
 }
 
 // ---------------------------------------------------------------------------
-// S of many tokens, on the tensor cores: 128 tokens (the M of the instruction) against the adapters among them (N: `width`
-// columns an adapter, its rank to a multiple of 16), K split over the CTAs of a cluster.  Each token keeps the columns of
-// its own adapter; the tile's list of adapters is walked in passes of `per_pass` (128 columns of TMEM).  With prompts a
-// tile has one or two adapters and X is read once; bound then: the bytes of X.
+// S of many tokens, on the tensor cores: the A matrices of 128 / rank adapters (the M of the instruction) against 128
+// tokens (N), K split over the CTAs of a cluster.  Each token keeps the rows of its own adapter; the tile's list of
+// adapters is walked in passes.  With prompts a tile has one or two adapters and X is read once; bound then: the bytes of
+// X.  (An instruction costs its issuer the same whatever its N, so the adapters share one; with the tokens as M and one
+// instruction an adapter, 16384 x 8192 tokens of 40 requests at rank 64 took 94 us.)
 //
-// Warp 0 copies by TMA (X 128 x 64 and `width` x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the
-// MMAs, warps 2..5 bring the accumulator (one token a lane) into shared memory, over the stages that have been used up.
+// Warp 0 copies by TMA (X 128 x 64 and rank x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the MMAs,
+// warps 2..5 bring the accumulator (one row of an A a lane) into shared memory, over the stages that have been used up.
 // The CTAs of the cluster then add the partial sums of 128 / cluster tokens each through distributed shared memory, in
 // the order of the ranks, and write them with one rounding: no atomics, no partial sums in memory.
 // ---------------------------------------------------------------------------
 constexpr int kShrinkTokens = 128, kShrinkStages = 3, kShrinkThreads = 192, kShrinkColumns = 128;
-constexpr int kShrinkXBytes = kShrinkTokens * 128, kShrinkABytes = kShrinkColumns * 128;
+constexpr int kShrinkXBytes = kShrinkTokens * 128, kShrinkABytes = 128 * 128;
 constexpr int kShrinkStageBytes = kShrinkXBytes + kShrinkABytes;
 constexpr int kShrinkSmem = kShrinkStages * kShrinkStageBytes + 1024 + 128;
 static_assert(kShrinkTokens * (kLoraMaxRank + 1) * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
@@ -196,21 +207,10 @@ __device__ __forceinline__ float cluster_load(uint32_t local, int rank)   // the
     asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
-{
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-
 __global__ void __launch_bounds__(kShrinkThreads, 2)
 lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const int *tiles,
-                        const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int adapters, int rank, int width,
-                        int per_pass, int kblocks, int split, int *status)
+                        const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int adapters, int rank, int per_pass,
+                        int kblocks, int split, int *status)
 {
     extern __shared__ unsigned char smem_dyn[];
     __shared__ int ids[kShrinkTokens], list[kShrinkTokens];   // adapter of each token; the adapters of the tile
@@ -276,11 +276,11 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
             for (int kb = kb0; kb < kb1 && ok; ++kb, ++i2) {
                 const int s = i2 % kShrinkStages;
                 if (!mbar_wait(empty_bar(s), ((i2 / kShrinkStages) & 1u) ^ 1u, abort_flag, status)) { ok = false; break; }
-                mbar_expect_tx(full_bar(s), (uint32_t)(kShrinkXBytes + n * width * 128));
+                mbar_expect_tx(full_bar(s), (uint32_t)(kShrinkXBytes + n * rank * 128));
                 const uint32_t sa = base + s * kShrinkStageBytes;
                 tma_load_3d(sa, &tmX, kb * 64, t0, 0, full_bar(s));
                 for (int a = 0; a < n; ++a)
-                    tma_load_3d(sa + kShrinkXBytes + a * width * 128, &tmA, kb * 64, 0, list[first + a], full_bar(s));
+                    tma_load_3d(sa + kShrinkXBytes + a * rank * 128, &tmA, kb * 64, 0, list[first + a], full_bar(s));
             }
             if (!ok) {   // copies on their way still land in this CTA's shared memory: give them time
                 const uint32_t pending = i2 < (uint32_t)kShrinkStages ? i2 : (uint32_t)kShrinkStages;
@@ -290,20 +290,18 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
                 }
             }
         } else if (warp == 1 && lane == 0) {
-            const uint32_t idesc = umma_idesc_bf16(kShrinkTokens, width);
+            constexpr uint32_t idesc = umma_idesc_bf16(128, kShrinkTokens);
             uint32_t i2 = it;
             for (int kb = kb0; kb < kb1; ++kb, ++i2) {
                 const int s = i2 % kShrinkStages;
                 if (!mbar_wait(full_bar(s), (i2 / kShrinkStages) & 1u, abort_flag, status)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t sa = base + s * kShrinkStageBytes;
-                const uint64_t xdesc = umma_desc_k_sw128(sa);
-                for (int a = 0; a < n; ++a) {
-                    const uint64_t adesc = umma_desc_k_sw128(sa + kShrinkXBytes + a * width * 128);
+                // rows of the A operand behind the adapters' hold whatever was there: their sums are not read
+                const uint64_t xdesc = umma_desc_k_sw128(sa), adesc = umma_desc_k_sw128(sa + kShrinkXBytes);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_bf16_ss(tmem + a * width, xdesc + 2 * k, adesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
-                }
+                for (int k = 0; k < 4; ++k)
+                    umma_bf16_ss(tmem, adesc + 2 * k, xdesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
                 umma_commit(empty_bar(s));
             }
             if (ok) umma_commit(done_bar);
@@ -314,20 +312,16 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
         ok = __syncthreads_and(ok && mbar_wait(done_bar, passes & 1u, abort_flag, status));
         if (ok && warp >= 2) {
             tc_fence_after();
-            const int q = warp & 3, row = q * 32 + lane;
-            const int id = ids[row];
-            for (int a = 0; a < n; ++a) {
-                const bool mine = id == list[first + a];
-                if (!__any_sync(0xffffffffu, mine)) continue;
-                for (int c = 0; c < rank; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + a * width + c, v);
-                    tmem_ld_wait();
-                    if (mine)
+            const int q = warp & 3, row = q * 32 + lane, a = row / rank, r = row - a * rank;
+            const int id = a < n ? list[first + a] : -1;   // -1 (no adapter) is no token's that is looked for here
+#pragma unroll 1
+            for (int c = 0; c < kShrinkTokens; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+                tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (c + i < rank) partial[row * pitch + c + i] = __uint_as_float(v[i]);
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (a < n && ids[c + i] == id) partial[(c + i) * pitch + r] = __uint_as_float(v[i]);
             }
             tc_fence_before();
         }
@@ -384,11 +378,11 @@ constexpr int kShrinkTileMin = 65;
 static int launch_shrink_tiles(const void *X, const void *A, const int *index, const float *scaling, const int *tiles,
                                __nv_bfloat16 *S, int tokens, int K, int adapters, int rank, cudaStream_t st)
 {
-    const int width = (rank + 15) & ~15, per_pass = kShrinkColumns / width;
+    const int per_pass = 128 / rank;
     CUtensorMap tx, ta;
     int rc = encode_tmap_bf16_stack(&tx, X, 1, (uint64_t)tokens, (uint64_t)K, kShrinkTokens);
     if (rc) return rc;
-    rc = encode_tmap_bf16_stack(&ta, A, (uint64_t)adapters, (uint64_t)rank, (uint64_t)K, (uint32_t)width);
+    rc = encode_tmap_bf16_stack(&ta, A, (uint64_t)adapters, (uint64_t)rank, (uint64_t)K, (uint32_t)rank);
     if (rc) return rc;
     rc = ensure_dyn_smem((const void *)lora_shrink_tile_kernel, kShrinkSmem);
     if (rc) return rc;
@@ -414,8 +408,8 @@ static int launch_shrink_tiles(const void *X, const void *A, const int *index, c
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, lora_shrink_tile_kernel, tx, ta, tiles, index, scaling, S, tokens, adapters, rank, width,
-                                   per_pass, K / 64, split, status_word_ptr());
+    return (int)cudaLaunchKernelEx(&cfg, lora_shrink_tile_kernel, tx, ta, tiles, index, scaling, S, tokens, adapters, rank, per_pass,
+                                   K / 64, split, status_word_ptr());
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
