@@ -96,7 +96,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.b200ht_lora_gemm.restype = i
     lib.b200ht_lora_gemm.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, f, vp, vp, sz, vp]
     lib.b200ht_lora_gemv_workspace_bytes.restype = sz
-    lib.b200ht_lora_gemv_workspace_bytes.argtypes = [i, i, i]
+    lib.b200ht_lora_gemv_workspace_bytes.argtypes = [i, i, i, i]
     lib.b200ht_lora_gemv.restype = i
     lib.b200ht_lora_gemv.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, vp, sz, vp]
     lib.b200ht_ipc_export.restype = i

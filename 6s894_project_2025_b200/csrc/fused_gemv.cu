@@ -18,6 +18,7 @@
 
 #include "tc_common.cuh"
 #include "fwht_f32.cuh"
+#include "lora.cuh"
 
 namespace b200ht {
 
@@ -288,12 +289,25 @@ struct PeerOut {
     int row_begin, rows_total;          // this rank's first row in the full result, rows of the full result
 };
 
-template <int NT, int GW>
+// Kernel argument of the form with adapters (b200ht_lora_gemv); nothing without.
+template <bool ADAPT>
+struct GemvAdaptArg {};
+template <>
+struct GemvAdaptArg<true> {
+    GemvAdapt a;
+};
+
+// With ADAPT, X is H(X) already (b-major: [column][N], made by lora_front_kernel) and arrives by bulk copies, while the
+// ring of W fills: the kernel in front releases this one only after all earlier work is complete, so W, B and index may
+// be read at once, and only X and S wait for it.  Each result gains B S of its column before it is rounded; these are
+// computed for kExtraFloats results at a time, the first of them while H(X) arrives.
+constexpr int kExtraFloats = 2048;
+template <int NT, int GW, bool ADAPT>
 __global__ void __launch_bounds__(GV_THREADS, 1)
 gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bfloat16 *X, void *Y, int M, int N,
                         int logn, int B, int b0, int Bg, int out_dtype, float scale, int rows_per_cta,
                         int group_rows, int kc, int stage_bytes, int nstages, int red_in_ring, int *status,
-                        const PeerOut po)
+                        const PeerOut po, const GemvAdaptArg<ADAPT> adapt)
 {
     extern __shared__ unsigned char smem_dyn[];
     // ring first (1024-byte aligned stages for the 128-byte swizzle), then H(X), reduction buffer, barriers
@@ -320,12 +334,15 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
     const int ngroups = (my_rows + group_rows - 1) / group_rows;
     const int nchunks = (N / 64) / kc;     // ring items per row group
     const int total_items = ngroups * nchunks;
+    float *extra = (float *)(bar_mem + 16 * nstages + 32);   // ADAPT: B S of the next results, [row][column]
+    const int extra_groups = kExtraFloats / (group_rows * Bg);
 
     if (tid == 0) {
         for (int s = 0; s < nstages; ++s) {
             mbar_init(full_bar(s), 1);
             released[s] = 0;
         }
+        if (ADAPT) mbar_init(bar_s + 16u * nstages + 8u, 1);   // H(X) is here
         *abort_flag = 0;
         fence_barrier_init();
         tma_prefetch_desc(&tmW);
@@ -335,12 +352,12 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
     // prefetch of X into L2 (a hint that returns no data, so it may run before the predecessor's writes are
     // visible; it warms the address translation for the loads below).
     pdl_launch_dependents();
-    {
+    if (!ADAPT) {
         const size_t xbytes = (size_t)N * B * 2;
         for (size_t off = (size_t)tid * 128; off < xbytes; off += (size_t)GV_THREADS * 128)
             asm volatile("prefetch.global.L2 [%0];\n" ::"l"((const unsigned char *)X + off));
+        pdl_wait();
     }
-    pdl_wait();
     // row-sharded call: the number of the call tags every value sent to a peer (read now, used at the end)
     unsigned int tag = po.target;
     if (po.n && tag == 0u) {
@@ -367,7 +384,27 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
     // ------------------------------ X^T into shared memory ------------------------------
     // Every path issues all loads of a batch before the first store: a round trip to memory is long while the
     // ring is filling, so the copy should cost one of them.
-    if (B == 1) {
+    if constexpr (ADAPT) {
+        if (warp == 0 && lane < (total_items < nstages ? total_items : nstages)) issue(lane);   // nstages <= 16
+        // this CTA's rows of the columns' B on their way to L2
+        for (int c = warp; c < Bg; c += GV_WARPS) {
+            const int a = adapt.a.index[b0 + c];
+            if ((unsigned)a >= (unsigned)adapt.a.adapters) continue;
+            const unsigned char *rows = (const unsigned char *)adapt.a.B + ((size_t)a * M + row_begin) * adapt.a.rank * 2;
+            for (int off = lane * 128; off < my_rows * adapt.a.rank * 2; off += 32 * 128)
+                asm volatile("prefetch.global.L2 [%0];\n" ::"l"(rows + off));
+        }
+        pdl_wait();
+        const uint32_t hx_bar = bar_s + 16u * nstages + 8u;
+        if (tid == 0) {
+            mbar_expect_tx(hx_bar, (uint32_t)(Bg * N * 2));
+            for (int c = 0; c < Bg; ++c)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                                 smem_u32(hxT) + (uint32_t)(c * pitch)),
+                             "l"(X + (size_t)(b0 + c) * N), "r"(N * 2), "r"(hx_bar)
+                             : "memory");
+        }
+    } else if (B == 1) {
         const uint4 *Xv = (const uint4 *)X;
         for (int base = 0; base < N / 8; base += GV_THREADS * 2) {
             uint4 r[2];
@@ -487,8 +524,8 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
             }
         }
     }
-    __syncthreads();
-    {
+    if (!ADAPT) {
+        __syncthreads();
         // pass A covers 8 + ra bits, pass B the remaining jb (N <= 8192: jb <= 3)
         const int ra = logn - 8 < 2 ? logn - 8 : 2;
         const int jb = logn - 8 - ra;
@@ -526,6 +563,46 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
     constexpr int UNR = NT <= 2 ? 4 : 2;
     const int ksteps = kc * 4;
     for (int grp = 0; grp < ngroups; ++grp) {
+        if constexpr (ADAPT) {
+            if (grp % extra_groups == 0) {
+                // rank / 8 lanes (to a power of two) a row of B, so that a warp reads neighbouring rows of one column's
+                // adapter; the last use of the buffer lies behind the barrier that ends a group
+                const int rank = adapt.a.rank, first = row_begin + grp * group_rows;
+                const int n = row_end - first < extra_groups * group_rows ? row_end - first : extra_groups * group_rows;
+                int lanes = 1;
+                while (lanes * 8 < rank) lanes *= 2;
+                const int j = lane % lanes, sub = lane / lanes, step = 32 / lanes;
+                const int blocks = (n + 4 * step - 1) / (4 * step);   // a warp's task: 4 * step rows of one column
+                for (int task = warp; task < blocks * Bg; task += GV_WARPS) {
+                    const int c = task % Bg, r0 = task / Bg * 4 * step + sub;
+                    const int a = adapt.a.index[b0 + c];
+                    const bool some = (unsigned)a < (unsigned)adapt.a.adapters && 8 * j < rank;
+                    const uint4 *bv = (const uint4 *)((const __nv_bfloat16 *)adapt.a.B + ((size_t)(some ? a : 0) * M + first) * rank) + j;
+                    float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
+                    uint4 p[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = r0 + u * step;
+                        p[u] = some && r < n ? bv[(size_t)r * (rank / 8)] : make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    if (some) {
+                        s0 = *(const float4 *)(adapt.a.S + (size_t)(b0 + c) * rank + 8 * j);
+                        s1 = *(const float4 *)(adapt.a.S + (size_t)(b0 + c) * rank + 8 * j + 4);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float2 u0 = unpack2<B200HT_BF16>(p[u].x), u1 = unpack2<B200HT_BF16>(p[u].y),
+                                     u2 = unpack2<B200HT_BF16>(p[u].z), u3 = unpack2<B200HT_BF16>(p[u].w);
+                        float v = fmaf(u0.x, s0.x, fmaf(u0.y, s0.y, fmaf(u1.x, s0.z, u1.y * s0.w)));
+                        v = fmaf(u2.x, s1.x, fmaf(u2.y, s1.y, fmaf(u3.x, s1.z, fmaf(u3.y, s1.w, v))));
+                        for (int o = lanes / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                        if (j == 0 && r0 + u * step < n) extra[(r0 + u * step) * Bg + c] = v;
+                    }
+                }
+                if (grp == 0 && !mbar_wait(bar_s + 16u * nstages + 8u, 0u, abort_flag, status)) return;
+                __syncthreads();
+            }
+        }
         float acc[2][NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -626,6 +703,7 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
             for (int w = 0; w < 8; ++w) sum += red[((size_t)w * 32 + r) * RC + c];
             const int row = grp_row0 + r;
             if (r < group_rows && row < row_end) {
+                if (ADAPT) sum += extra[(grp % extra_groups * group_rows + r) * Bg + c];
                 store_out(Y, (size_t)row * B + b0 + c, sum, out_dtype);
                 // the same value, with the call's tag beside it, into the slot arrays of the other ranks: one 8-byte
                 // store each, which arrives whole, so a peer that reads the tag has the value
@@ -767,12 +845,12 @@ static int launch_bf16_nt(const void *W, const void *X, void *Y, int M, int N, i
 }
 
 constexpr size_t kStreamSmemLimit = 225 * 1024;
-static size_t stream_fixed_smem(int N, int cols, bool red_in_ring = false)
+static size_t stream_fixed_smem(int N, int cols, bool red_in_ring = false, bool adapt = false)
 {
     const int nt = (cols + 7) / 8;
     return (((size_t)cols * hxt_pitch(N) + 127) & ~(size_t)127) +
            (red_in_ring ? 0 : (size_t)(GV_WARPS / 2) * 32 * nt * 8 * 4) + 1024 /*alignment*/ + 16 * 16 +
-           64 /*barriers, counters*/;
+           64 /*barriers, counters*/ + (adapt ? kExtraFloats * sizeof(float) : 0);
 }
 // Columns per launch on the fast path (all of B, or a multiple of 8), 0 if the shape does not take it
 // (the ring needs room for at least 64 KB).
@@ -784,9 +862,9 @@ static int stream_cols_max(int N, int B)
     return stream_fixed_smem(N, cols) + 64 * 1024 <= kStreamSmemLimit ? cols : 0;
 }
 
-template <int NT>
+template <int NT, bool ADAPT>
 static int launch_stream_nt(const void *W, const void *X, void *Y, int M, int N, int logn, int B, int b0, int Bg,
-                            int out_dtype, float scale, cudaStream_t st, const PeerOut &po)
+                            int out_dtype, float scale, cudaStream_t st, const PeerOut &po, const GemvAdaptArg<ADAPT> &adapt)
 {
     // one CTA per SM, but never fewer than 8 rows per CTA
     int grid = sm_count();
@@ -806,7 +884,7 @@ static int launch_stream_nt(const void *W, const void *X, void *Y, int M, int N,
     int wgroups = 4, only_kc = 0;
     int kc = 0, stages = 0, stage_bytes = 0;
     auto plan = [&](bool red_in_ring) {
-        const size_t ring_room = kStreamSmemLimit - stream_fixed_smem(N, Bg, red_in_ring);
+        const size_t ring_room = kStreamSmemLimit - stream_fixed_smem(N, Bg, red_in_ring, ADAPT);
         size_t best = 0;
         kc = 0;
         // (kc = 4 first: with four warps per group it is the one-batch-per-warp cut, so it wins ties)
@@ -842,28 +920,42 @@ static int launch_stream_nt(const void *W, const void *X, void *Y, int M, int N,
         }
     }
     if (!kc) return B200HT_ERR_SIZE;
-    const size_t smem = stream_fixed_smem(N, Bg, red_in_ring) + (size_t)stages * stage_bytes;
+    const size_t smem = stream_fixed_smem(N, Bg, red_in_ring, ADAPT) + (size_t)stages * stage_bytes;
     CUtensorMap tw;
     int rc = encode_tmap_bf16_rows_chunks(&tw, W, (uint64_t)M, (uint64_t)N, (uint32_t)group_rows, (uint32_t)kc);
     if (rc) return rc;
-    auto kernel = wgroups == 4 ? gemv_bf16_stream_kernel<NT, GV_WARPS / 4> : gemv_bf16_stream_kernel<NT, GV_WARPS / 2>;
+    auto kernel = wgroups == 4 ? gemv_bf16_stream_kernel<NT, GV_WARPS / 4, ADAPT> : gemv_bf16_stream_kernel<NT, GV_WARPS / 2, ADAPT>;
     rc = ensure_dyn_smem((const void *)kernel, (int)smem);
     if (rc) return rc;
     return launch_pdl(kernel, dim3(grid), dim3(GV_THREADS), smem, st, tw, (const __nv_bfloat16 *)X, Y, M, N, logn, B, b0,
                       Bg, out_dtype, scale, rows_per_cta, group_rows, kc, stage_bytes, stages, red_in_ring ? 1 : 0,
-                      status_word_ptr(), po);
+                      status_word_ptr(), po, adapt);
 }
 
+template <bool ADAPT = false>
 static int launch_stream(const void *W, const void *X, void *Y, int M, int N, int logn, int B, int b0, int Bg,
-                         int out_dtype, float scale, cudaStream_t st, const PeerOut &po = PeerOut{})
+                         int out_dtype, float scale, cudaStream_t st, const PeerOut &po = PeerOut{},
+                         const GemvAdaptArg<ADAPT> &adapt = GemvAdaptArg<ADAPT>{})
 {
     switch ((Bg + 7) / 8) {
-    case 1: return launch_stream_nt<1>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po);
-    case 2: return launch_stream_nt<2>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po);
-    case 3: return launch_stream_nt<3>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po);
-    case 4: return launch_stream_nt<4>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po);
+    case 1: return launch_stream_nt<1, ADAPT>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po, adapt);
+    case 2: return launch_stream_nt<2, ADAPT>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po, adapt);
+    case 3: return launch_stream_nt<3, ADAPT>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po, adapt);
+    case 4: return launch_stream_nt<4, ADAPT>(W, X, Y, M, N, logn, B, b0, Bg, out_dtype, scale, st, po, adapt);
     }
     return B200HT_ERR_SIZE;
+}
+
+// W . Xt + B S in one launch (see the kernel); shapes whose columns all fit beside the stream of W.
+bool gemv_adapt_shape(int N, int B)
+{
+    const int most = stream_cols_max(N, B);
+    return most > 0 && B <= most;
+}
+int launch_gemv_adapt(const void *W, const void *Xt, void *Y, int M, int N, int B, int out_dtype, const GemvAdapt &adapt,
+                      cudaStream_t st)
+{
+    return launch_stream<true>(W, Xt, Y, M, N, ilog2((uint32_t)N), B, 0, B, out_dtype, 1.f, st, PeerOut{}, GemvAdaptArg<true>{adapt});
 }
 
 static size_t bf16_smem(int N, int Bg, int gc)

@@ -3,10 +3,13 @@
 // a = index[t] the adapter of token t (none where it lies outside 0 .. adapters - 1).  The adapter sees the token as the
 // caller gives it, without H: an adapter trained beside the unrotated weight keeps its matrices.
 //
+//   H(X)                  lora_transform_kernel: fp32 throughout, one rounding to bf16
 //   S = s_a * A_a x_t     lora_shrink_rows_kernel (few tokens: a block per token and some rows of A) or
 //                         lora_shrink_tile_kernel (tcgen05: 128 tokens against the adapters among them)
 //   C = W . H(X) + B S    prompts: further K steps of the contraction itself (gemm_tcgen05.cu), one rounding;
-//                         decoding: fused GEMV into fp32, then lora_expand_kernel adds B S and rounds
+//                         decoding: lora_front_kernel (H(X) and S in one launch), then the streaming GEMV, which adds
+//                         B S to its sums (fused_gemv.cu); shapes that do not take it: fused GEMV into fp32, then
+//                         lora_expand_kernel adds B S and rounds
 // Sums are fp32; S is rounded to bf16 where it becomes an operand of the tensor cores (like H(X) itself), and stays fp32
 // when decoding.  There is no counterpart in the reference.
 #include "lora.cuh"
@@ -17,8 +20,18 @@ namespace b200ht {
 int launch_fwht(const void *in, void *out, uint64_t rows, uint32_t n, int dtype, float scale, const void *signs,
                 cudaStream_t st, int keep_out);
 int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1);
+int launch_gemv_adapt(const void *W, const void *Xt, void *Y, int M, int N, int B, int out_dtype, const GemvAdapt &adapt,
+                      cudaStream_t st);
+bool gemv_adapt_shape(int N, int B);
 int fused_gemm_bf16_lora(const void *X, const void *W, void *C, int M, int N, int K, int out_dtype, int out_layout, float scale,
                          const void *signs, void *workspace, cudaStream_t st, const LoraGemm &lora);
+
+// All threads of all CTAs of the cluster.
+__device__ __forceinline__ void cluster_sync_all()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
 
 // ---------------------------------------------------------------------------
 // Which adapters occur in each tile of tokens.  A token whose adapter no earlier token of the tile has opens its entry
@@ -78,32 +91,163 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
 }
 
 // ---------------------------------------------------------------------------
-// S of few tokens: blockIdx.x the token, blockIdx.y a group of `rows` rows of its A; 8 / rows warps share a row.  Bound:
-// the bytes of A (rank * K * 2 a token; tokens of one adapter share them through L2).  x comes from global memory where
-// its elements are contiguous, else (b fastest, more than one column) through shared memory.
+// H of one token by one block, in fp32 with one rounding at the end (the transform of fwht.cu passes 16-bit values between
+// its stages, two or three roundings more; beside adapters, whose share of the result is small, they would be the larger
+// error).  The row lies in shared memory as fp32 lines of 32 values, their 16-byte pieces exchanged by the line's number
+// so that no access below meets bank conflicts:
+//   A  32 consecutive values a thread from global memory: bits 0 .. 4 of the index
+//   B  rounds of up to five bits from bit 5 on, lanes side by side
+//   C  8 consecutive values and the last two bits: scaled, rounded, stored as 16-byte vectors
+// `stride`: distance of two elements of the token.
 // ---------------------------------------------------------------------------
-template <bool CONTIGUOUS, typename OUT>
-__global__ void __launch_bounds__(256)
-lora_shrink_rows_kernel(const __nv_bfloat16 *X, const __nv_bfloat16 *A, const int *index, const float *scaling, OUT *S, int tokens,
-                        int K, int adapters, int rank, int rows)
+__device__ __forceinline__ int line_at(int e)   // place of element e
 {
-    extern __shared__ __align__(16) __nv_bfloat16 xs[];
-    __shared__ float part[8];
+    const int line = e >> 5;
+    return (line << 5) | ((((e >> 2) ^ line) & 7) << 2) | (e & 3);
+}
+template <int BITS>
+__device__ __forceinline__ void fwht_round(float *row, int K, int bit)   // bits bit .. bit + BITS - 1, bit >= 5
+{
+    for (int task = threadIdx.x; task < (K >> BITS); task += blockDim.x) {
+        const int e0 = ((task >> bit) << (bit + BITS)) | (task & ((1 << bit) - 1));
+        float v[1 << BITS];
+#pragma unroll
+        for (int i = 0; i < (1 << BITS); ++i) v[i] = row[line_at(e0 + (i << bit))];
+#pragma unroll
+        for (int m = 1; m < (1 << BITS); m <<= 1)
+#pragma unroll
+            for (int i = 0; i < (1 << BITS); ++i)
+                if (!(i & m)) {
+                    const float a = v[i], b = v[i | m];
+                    v[i] = a + b;
+                    v[i | m] = a - b;
+                }
+#pragma unroll
+        for (int i = 0; i < (1 << BITS); ++i) row[line_at(e0 + (i << bit))] = v[i];
+    }
+    __syncthreads();
+}
+template <int BITS>
+__device__ __forceinline__ void fwht_last(const float *row, __nv_bfloat16 *out, int K, float scale)
+{
+    constexpr int N = 1 << BITS;
+    const int step = K >> BITS;
+    for (int task = threadIdx.x; task < step / 8; task += blockDim.x) {
+        float v[N][8];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 f = *(const float4 *)(row + line_at(task * 8 + i * step + 4 * h));
+                v[i][4 * h] = f.x, v[i][4 * h + 1] = f.y, v[i][4 * h + 2] = f.z, v[i][4 * h + 3] = f.w;
+            }
+#pragma unroll
+        for (int m = 1; m < N; m <<= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (!(i & m))
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float a = v[i][e], b = v[i | m][e];
+                        v[i][e] = a + b;
+                        v[i | m][e] = a - b;
+                    }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            *(uint4 *)(out + task * 8 + i * step) =
+                make_uint4(pack2<B200HT_BF16>(v[i][0] * scale, v[i][1] * scale), pack2<B200HT_BF16>(v[i][2] * scale, v[i][3] * scale),
+                           pack2<B200HT_BF16>(v[i][4] * scale, v[i][5] * scale), pack2<B200HT_BF16>(v[i][6] * scale, v[i][7] * scale));
+    }
+}
+// K = 2^logk >= 64; x: the token's first element; out: K values; signs: 0x8000 where an element is negated, or NULL.
+__device__ __forceinline__ void fwht_token(float *row, const __nv_bfloat16 *x, int stride, __nv_bfloat16 *out, int logk, float scale,
+                                           const uint16_t *signs)
+{
+    const int K = 1 << logk;
+    for (int task = threadIdx.x; task < K / 32; task += blockDim.x) {
+        float v[32];
+        if (stride == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 p = ((const uint4 *)(x + task * 32))[i];
+                if (signs) {
+                    const uint4 sg = ((const uint4 *)(signs + task * 32))[i];
+                    p.x ^= sg.x, p.y ^= sg.y, p.z ^= sg.z, p.w ^= sg.w;
+                }
+                const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = unpack2<B200HT_BF16>(w[e]);
+                    v[8 * i + 2 * e] = f.x;
+                    v[8 * i + 2 * e + 1] = f.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __bfloat162float(x[(size_t)(task * 32 + i) * stride]);
+        }
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (!(i & m)) {
+                    const float a = v[i], b = v[i | m];
+                    v[i] = a + b;
+                    v[i | m] = a - b;
+                }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *(float4 *)(row + line_at(task * 32 + 4 * i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+    __syncthreads();
+    const int last = logk >= 7 ? 2 : 1;
+    for (int bit = 5, left = logk - 5 - last; left > 0;) {
+        const int n = left <= 5 ? left : (left + 1) / 2;
+        if (n == 1) fwht_round<1>(row, K, bit);
+        else if (n == 2) fwht_round<2>(row, K, bit);
+        else if (n == 3) fwht_round<3>(row, K, bit);
+        else if (n == 4) fwht_round<4>(row, K, bit);
+        else fwht_round<5>(row, K, bit);
+        bit += n;
+        left -= n;
+    }
+    if (last == 2) fwht_last<2>(row, out, K, scale);
+    else fwht_last<1>(row, out, K, scale);
+}
+
+__global__ void __launch_bounds__(512) lora_transform_kernel(const __nv_bfloat16 *X, __nv_bfloat16 *Y, int logk, float scale,
+                                                             const uint16_t *signs)
+{
+    extern __shared__ __align__(16) unsigned char smem_row[];
     pdl_launch_dependents();
     pdl_wait();
-    const int t = blockIdx.x, r0 = blockIdx.y * rows;
-    const int a = index[t];
+    const size_t at = (size_t)blockIdx.x << logk;
+    fwht_token((float *)smem_row, X + at, 1, Y + at, logk, scale, signs);
+}
+
+// ---------------------------------------------------------------------------
+// S of few tokens: a block takes `rows` rows of a token's A; 8 / rows warps share a row.  Bound: the bytes of A
+// (rank * K * 2 a token; tokens of one adapter share them through L2).  x comes from global memory where its elements are
+// contiguous, else (b fastest, more than one column) through shared memory.
+// ---------------------------------------------------------------------------
+template <typename OUT>
+__device__ __forceinline__ void shrink_rows(const __nv_bfloat16 *X, int stride, size_t token_at, const __nv_bfloat16 *A, int a, bool some,
+                                            const float *scaling, OUT *S, __nv_bfloat16 *xs, int K, int rank, int r0, int rows)
+{   // `rank`: rows of A; S: the token's
+    __shared__ float part[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = 8 / rows, r = r0 + warp / share;   // warps of a row; this warp's row
-    const bool some = (unsigned)a < (unsigned)adapters;
-    if (!CONTIGUOUS && some)
-        for (int k = threadIdx.x; k < K; k += 256) xs[k] = X[(size_t)k * tokens + t];
-    __syncthreads();
+    if (stride != 1) {
+        if (some)
+#pragma unroll 8
+            for (int k = threadIdx.x; k < K; k += 256) xs[k] = X[token_at + (size_t)k * stride];
+        __syncthreads();
+    }
     float acc = 0.f;
     if (some && r < rank) {
         const uint4 *av = (const uint4 *)(A + ((size_t)a * rank + r) * K);
-        const uint4 *xv = CONTIGUOUS ? (const uint4 *)(X + (size_t)t * K) : (const uint4 *)xs;
-#pragma unroll 4
+        const uint4 *xv = stride == 1 ? (const uint4 *)(X + token_at) : (const uint4 *)xs;
+#pragma unroll 8
         for (int v = (warp % share) * 32 + lane; v < K / 8; v += share * 32) {
             const uint4 p = av[v], q = xv[v];
             const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
@@ -122,9 +266,78 @@ lora_shrink_rows_kernel(const __nv_bfloat16 *X, const __nv_bfloat16 *A, const in
         float s = 0.f;
         for (int w = 0; w < share; ++w) s += part[threadIdx.x * share + w];
         if (some && scaling) s *= scaling[a];
-        OUT *o = S + (size_t)t * rank + r0 + threadIdx.x;
-        if constexpr (sizeof(OUT) == 4) *o = s;
-        else *o = __float2bfloat16_rn(s);
+        if constexpr (sizeof(OUT) == 4) S[r0 + threadIdx.x] = s;
+        else S[r0 + threadIdx.x] = __float2bfloat16_rn(s);
+    }
+}
+
+// stride: distance of two elements of a token; token t begins at t * (stride == 1 ? K : 1).
+template <typename OUT>
+__global__ void __launch_bounds__(256)
+lora_shrink_rows_kernel(const __nv_bfloat16 *X, int stride, const __nv_bfloat16 *A, const int *index, const float *scaling, OUT *S,
+                        int K, int adapters, int rank, int rows)
+{
+    extern __shared__ __align__(16) unsigned char smem_row[];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = blockIdx.x, a = index[t];
+    shrink_rows<OUT>(X, stride, (size_t)t * (stride == 1 ? K : 1), A, a, (unsigned)a < (unsigned)adapters, scaling, S + (size_t)t * rank,
+                     (__nv_bfloat16 *)smem_row, K, rank, blockIdx.y * rows, rows);
+}
+
+// Decoding: H(X) and S of every column in one launch.  It lets the next kernel start only once it has itself seen all
+// earlier work complete, so the streaming GEMV behind it may read W, B and index at once and waits for nothing but Xt and S.
+//
+// One column (CLUSTER false): block 0 transforms, the others take `rows` rows of A each, x comes straight from memory.
+// Several columns: a cluster of eight CTAs a column.  The elements of a column lie a row of X apart, a 32-byte sector
+// each, so every CTA fetches an eighth and they exchange it through distributed shared memory (each fetching all of it,
+// 272 CTAs of a batch of 16 at N = 4096 moved 35 MB through L2 and took 8 us).  Rank 0 transforms, the others divide A.
+template <bool CLUSTER>
+__global__ void __launch_bounds__(256)
+lora_front_kernel(const __nv_bfloat16 *X, const __nv_bfloat16 *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S,
+                  int columns, int logk, float scale, int adapters, int rank, int rows)
+{
+    extern __shared__ __align__(16) unsigned char smem_row[];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int K = 1 << logk;
+    if constexpr (!CLUSTER) {
+        if (blockIdx.x == 0) {
+            fwht_token((float *)smem_row, X, 1, Xt, logk, scale, nullptr);
+        } else {
+            const int a = index[0];
+            shrink_rows<float>(X, 1, 0, A, a, (unsigned)a < (unsigned)adapters, scaling, S, nullptr, K, rank, (blockIdx.x - 1) * rows, rows);
+        }
+        return;
+    }
+    __nv_bfloat16 *xs = (__nv_bfloat16 *)smem_row;   // the column; behind it the transform's fp32 row
+    const int column = blockIdx.x / 8, part = blockIdx.x % 8, slice = K / 8;
+    const int a = index[column];
+    const __nv_bfloat16 *x = X + (size_t)part * slice * columns + column;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < slice; k += 256) xs[part * slice + k] = x[(size_t)k * columns];
+    cluster_sync_all();
+    for (int v = threadIdx.x; v < K / 8; v += 256) {
+        const int from = v / (slice / 8);
+        if (from == part) continue;
+        uint32_t at;
+        uint4 p;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(xs) + (uint32_t)v * 16), "r"(from));
+        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(p.x), "=r"(p.y), "=r"(p.z), "=r"(p.w) : "r"(at) : "memory");
+        ((uint4 *)xs)[v] = p;
+    }
+    cluster_sync_all();   // no CTA writes again what others read, and none has left before they have
+    if (part == 0) {
+        fwht_token((float *)(smem_row + K * 2), xs, 1, Xt + ((size_t)column << logk), logk, scale, nullptr);
+    } else {
+        const int per = (rank + 6) / 7, r0 = (part - 1) * per, r1 = r0 + per < rank ? r0 + per : rank;
+        const bool some = (unsigned)a < (unsigned)adapters;
+        for (int r = r0; r < r1; r += rows) {
+            shrink_rows<float>(xs, 1, 0, A + (some ? (size_t)a * rank * K : 0), 0, some, nullptr, S + (size_t)column * rank, nullptr, K, r1,
+                               r, rows);
+            __syncthreads();
+        }
+        if (some && scaling && (int)threadIdx.x < r1 - r0) S[(size_t)column * rank + r0 + threadIdx.x] *= scaling[a];
     }
 }
 
@@ -194,11 +407,6 @@ constexpr int kShrinkStageBytes = kShrinkXBytes + kShrinkABytes;
 constexpr int kShrinkSmem = kShrinkStages * kShrinkStageBytes + 1024 + 128;
 static_assert(kShrinkTokens * (kLoraMaxRank + 1) * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
 
-__device__ __forceinline__ void cluster_sync_all()
-{
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
 __device__ __forceinline__ float cluster_load(uint32_t local, int rank)   // the float at `local` in the shared memory of CTA `rank`
 {
     float v;
@@ -354,22 +562,54 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-template <typename OUT>
-static int launch_shrink_rows(const void *X, const void *A, const int *index, const float *scaling, OUT *S, int tokens, int K,
-                              int adapters, int rank, bool contiguous, cudaStream_t st)
+// launch_pdl with clusters of `cluster` CTAs along x.
+template <typename... KArgs, typename... Args>
+static int launch_pdl_cluster(void (*kernel)(KArgs...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args)
 {
-    // one row of A a block spreads a short call over the SMs; with enough tokens eight rows share the block's start
+    note_launch();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// Rows of A a block takes: one spreads a short call over the SMs; with enough tokens eight share the block's start.
+static int shrink_rows_of_block(int tokens, int rank)
+{
     int rows = 8;
     while (rows > 1 && (long)tokens * ((rank + rows - 1) / rows) < 2 * sm_count()) rows /= 2;
-    const dim3 grid((unsigned)tokens, (unsigned)((rank + rows - 1) / rows));
-    if (contiguous)
-        return launch_pdl(lora_shrink_rows_kernel<true, OUT>, grid, dim3(256), 0, st, (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A,
-                          index, scaling, S, tokens, K, adapters, rank, rows);
-    const size_t smem = (size_t)K * 2;
-    int rc = ensure_dyn_smem((const void *)lora_shrink_rows_kernel<false, OUT>, (int)smem);
+    return rows;
+}
+
+template <typename OUT>
+static int launch_shrink_rows(const void *X, const void *A, const int *index, const float *scaling, OUT *S, int tokens, int K,
+                              int adapters, int rank, int stride, cudaStream_t st)
+{
+    const int rows = shrink_rows_of_block(tokens, rank);
+    const size_t smem = stride == 1 ? 0 : (size_t)K * 2;
+    int rc = ensure_dyn_smem((const void *)lora_shrink_rows_kernel<OUT>, (int)smem);
     if (rc) return rc;
-    return launch_pdl(lora_shrink_rows_kernel<false, OUT>, grid, dim3(256), smem, st, (const __nv_bfloat16 *)X,
-                      (const __nv_bfloat16 *)A, index, scaling, S, tokens, K, adapters, rank, rows);
+    return launch_pdl(lora_shrink_rows_kernel<OUT>, dim3((unsigned)tokens, (unsigned)((rank + rows - 1) / rows)), dim3(256), smem, st,
+                      (const __nv_bfloat16 *)X, stride, (const __nv_bfloat16 *)A, index, scaling, S, K, adapters, rank, rows);
+}
+
+int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, cudaStream_t st)
+{
+    const int threads = K / 32 < 64 ? 64 : (K / 32 > 512 ? 512 : K / 32), smem = K * 4;
+    int rc = ensure_dyn_smem((const void *)lora_transform_kernel, smem);
+    if (rc) return rc;
+    return launch_pdl(lora_transform_kernel, dim3((unsigned)tokens), dim3((unsigned)threads), (size_t)smem, st, (const __nv_bfloat16 *)X,
+                      (__nv_bfloat16 *)Y, ilog2((uint32_t)K), scale, (const uint16_t *)signs);
 }
 
 // Tokens from which the tile kernel serves a prompt (see launch_shrink_tiles).
@@ -394,22 +634,30 @@ static int launch_shrink_tiles(const void *X, const void *A, const int *index, c
     const int most = adapters < kShrinkTokens ? adapters : kShrinkTokens, passes = (most + per_pass - 1) / per_pass;
     int ways = room / (ntiles * split);
     ways = ways < 1 ? 1 : (ways > passes ? passes : ways);
-    note_launch();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ntiles * split), (unsigned)ways);
-    cfg.blockDim = dim3(kShrinkThreads);
-    cfg.dynamicSmemBytes = kShrinkSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)split;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, lora_shrink_tile_kernel, tx, ta, tiles, index, scaling, S, tokens, adapters, rank, per_pass,
-                                   K / 64, split, status_word_ptr());
+    return launch_pdl_cluster(lora_shrink_tile_kernel, (unsigned)split, dim3((unsigned)(ntiles * split), (unsigned)ways),
+                              dim3(kShrinkThreads), (size_t)kShrinkSmem, st, tx, ta, tiles, index, scaling, S, tokens, adapters, rank,
+                              per_pass, K / 64, split, status_word_ptr());
+}
+
+static int launch_front(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S, int columns,
+                        int N, float scale, int adapters, int rank, cudaStream_t st)
+{
+    const int logk = ilog2((uint32_t)N);
+    if (columns == 1) {
+        const int rows = shrink_rows_of_block(1, rank), smem = N * 4;
+        int rc = ensure_dyn_smem((const void *)lora_front_kernel<false>, smem);
+        if (rc) return rc;
+        return launch_pdl(lora_front_kernel<false>, dim3((unsigned)(1 + (rank + rows - 1) / rows)), dim3(256), (size_t)smem, st,
+                          (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, 1, logk, scale, adapters, rank, rows);
+    }
+    int rows = 1;   // rows of A at a time, of the seventh that a CTA has
+    while (rows < 8 && rows < (rank + 6) / 7) rows *= 2;
+    const int smem = N * 2 + N * 4;
+    int rc = ensure_dyn_smem((const void *)lora_front_kernel<true>, smem);
+    if (rc) return rc;
+    return launch_pdl_cluster(lora_front_kernel<true>, 8, dim3((unsigned)columns * 8), dim3(256), (size_t)smem, st,
+                              (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, columns, logk, scale, adapters,
+                              rank, rows);
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -458,17 +706,18 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     rc = launch_pdl(lora_plan_kernel, dim3(ntiles), dim3(256), 0, st, index, N, adapters, tiles);
     if (rc) return rc;
     rc = N >= kShrinkTileMin ? launch_shrink_tiles(X, A, index, scaling, tiles, S, N, K, adapters, rank, st)
-                             : launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, true, st);
+                             : launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, 1, st);
     if (rc) return rc;
     const LoraGemm lora{B, S, tiles, index, adapters, M, rank, 0};
     return fused_gemm_bf16_lora(X, W, C, M, N, K, out_dtype, out_layout, scale, signs, workspace, st, lora);
 }
 
-extern "C" size_t b200ht_lora_gemv_workspace_bytes(int M, int B, int rank)
+extern "C" size_t b200ht_lora_gemv_workspace_bytes(int M, int N, int B, int rank)
 {
     using namespace b200ht;
-    if (M <= 0 || B <= 0 || rank <= 0) return 0;
-    return up256((size_t)M * B * sizeof(float)) + up256((size_t)B * rank * sizeof(float));
+    if (M <= 0 || N <= 0 || B <= 0 || rank <= 0) return 0;
+    const size_t base = gemv_adapt_shape(N, B) ? (size_t)N * B * 2 : (size_t)M * B * sizeof(float);   // H(X), or W . H(X)
+    return up256(base) + up256((size_t)B * rank * sizeof(float));
 }
 
 extern "C" int b200ht_lora_gemv(const void *W, const void *X, void *Y, const void *A, const void *Bm, const int *index,
@@ -484,13 +733,20 @@ extern "C" int b200ht_lora_gemv(const void *W, const void *X, void *Y, const voi
     if (!aligned16(W) || !aligned16(X) || !aligned16(Y) || !aligned16(A) || !aligned16(Bm) || ((uintptr_t)index & 3u) ||
         ((uintptr_t)scaling & 3u))
         return B200HT_ERR_ALIGN;
-    if (!workspace || workspace_bytes < b200ht_lora_gemv_workspace_bytes(M, B, rank)) return B200HT_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < b200ht_lora_gemv_workspace_bytes(M, N, B, rank)) return B200HT_ERR_WORKSPACE;
     if ((uintptr_t)workspace & 255u) return B200HT_ERR_ALIGN;
     rc = check_device();
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
+    if (gemv_adapt_shape(N, B)) {
+        __nv_bfloat16 *Xt = (__nv_bfloat16 *)workspace;
+        float *S = (float *)((unsigned char *)workspace + up256((size_t)N * B * 2));
+        rc = launch_front(X, A, index, scaling, Xt, S, B, N, scale, adapters, rank, st);
+        if (rc) return rc;
+        return launch_gemv_adapt(W, Xt, Y, M, N, B, out_dtype, GemvAdapt{Bm, S, index, adapters, rank}, st);
+    }
     float *base = (float *)workspace, *S = (float *)((unsigned char *)workspace + up256((size_t)M * B * sizeof(float)));
-    rc = launch_shrink_rows(X, A, index, scaling, S, B, N, adapters, rank, B == 1, st);
+    rc = launch_shrink_rows(X, A, index, scaling, S, B, N, adapters, rank, B, st);
     if (rc) return rc;
     rc = b200ht_fused_gemv(W, X, base, M, N, B, B200HT_BF16, B200HT_F32, scale, stream);
     if (rc) return rc;

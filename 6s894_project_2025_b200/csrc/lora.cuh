@@ -31,4 +31,12 @@ struct LoraGemm {
     }
 };
 
+// The adapters of a decoding batch, as the streaming GEMV takes them.
+struct GemvAdapt {
+    const void *B;       // [adapters][M][rank] bf16
+    const float *S;      // [columns][rank]
+    const int *index;    // adapter of each column
+    int adapters, rank;
+};
+
 }  // namespace b200ht

@@ -126,7 +126,7 @@ def lora_ht_gemv(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Ten
     out = _out("lora_ht_gemv", out, (M, columns), out_dtype, X.device)
     if M == 0:
         return out
-    ws = torch.empty(lib.b200ht_lora_gemv_workspace_bytes(M, columns, rank), dtype=torch.uint8, device=X.device)
+    ws = torch.empty(lib.b200ht_lora_gemv_workspace_bytes(M, N, columns, rank), dtype=torch.uint8, device=X.device)
     with _on_device(X.device):
         rc = lib.b200ht_lora_gemv(W.data_ptr(), X.data_ptr(), out.data_ptr(), A.data_ptr(), B.data_ptr(), index.data_ptr(),
                                   None if scaling is None else scaling.data_ptr(), M, N, columns, adapters, rank,

@@ -287,7 +287,7 @@ int b200ht_norm_rotary_qk_backward(const void *dq_out, const void *dk_out, const
  *   scaling  one float per adapter, or NULL for 1
  *   signs    as in b200ht_fused_gemm_signed, or NULL
  * K a power of two, 64 .. 32768; rank a multiple of 8, 8 .. 128 (pad with rows and columns of zeros).  W, X, A, B bf16;
- * the low-rank vectors are rounded to bf16 once, like H(X), everything else is accumulated in fp32.
+ * H(X) (fp32 throughout here) and the low-rank vectors are rounded to bf16 once, everything else is accumulated in fp32.
  * An adapter's B is multiplied with zeros for the other tokens of a group of 16 (tokens 16 i .. 16 i + 15) that has one
  * of its tokens: infinities or NaN in B reach those tokens too.  Adapters that no token names are not read.
  * `workspace`: b200ht_lora_gemm_workspace_bytes(M, N, K, rank) bytes, 256-byte aligned.  Calls that share one must not
@@ -301,9 +301,9 @@ int b200ht_lora_gemm(const void *X, const void *W, void *C, const void *A, const
 /*
  * The same for a decoding batch, in the layouts of b200ht_fused_gemv (bf16): X  N x B with b fastest, Y  M x B with b
  * fastest, index[b] the adapter of column b, 1 <= B <= 64, N a power of two, 64 .. 32768.  The low-rank vectors stay
- * fp32; one rounding.  `workspace`: b200ht_lora_gemv_workspace_bytes(M, B, rank) bytes, 256-byte aligned.
+ * fp32; one rounding.  `workspace`: b200ht_lora_gemv_workspace_bytes(M, N, B, rank) bytes, 256-byte aligned.
  */
-size_t b200ht_lora_gemv_workspace_bytes(int M, int B, int rank);
+size_t b200ht_lora_gemv_workspace_bytes(int M, int N, int B, int rank);
 int b200ht_lora_gemv(const void *W, const void *X, void *Y, const void *A, const void *Bm, const int *index,
                      const float *scaling, int M, int N, int B, int adapters, int rank, int out_dtype, float scale,
                      void *workspace, size_t workspace_bytes, void *stream);

@@ -1,15 +1,19 @@
-"""W . H(X) with the adapters of many requests, against the definition in 64 bits.
+"""W . H(X) with the adapters of many requests, against the definition in 64 bits, in two parts.
 
-The base product is tested elsewhere; here the adapters' share is looked at by itself, as the difference between a call
-with fp32 results and the same call without adapters (same transform, same order of the base's sums, so the base cancels
-up to the roundings named below).  With S_r = scaling * sum_k A_rk x_k the share is sum_r B_mr S_r.  Its error:
+Without adapters (every index -1) the result is W . H(X) with H(X) computed in fp32 and rounded to bf16 once: each of its
+K terms is off by at most 2^-8 of its size, plus the fp32 error of the transform (log2 K + 1 additions, 2^-24 each of the
+row's norm) and of the sum: the tensor cores add 16 products at a time and may cut instead of rounding, 2^-22 of the sizes'
+sum for each of the K / 16 additions.
 
-* S: a sum of K products in fp32, off by at most K units of 2^-24 of the sum of their sizes, however it is ordered; times
-  the scaling, one unit; for the tensor cores rounded to bf16, 2^-8 of its size;
-* B S: rank products (exact in fp32) added to a sum that already holds the base: the tensor cores add 16 products at a
-  time and may cut instead of rounding, so each of the rank / 16 + 1 additions is off by at most 2^-22 of the largest
-  size the sum can have; by fp32 arithmetic (decoding) rank + 2 additions by 2^-23 each;
-* the difference of the two results itself is fp64.
+With adapters, the difference from that call (fp32 results: the same transform, the same order of the base's sums, so the
+base cancels) is the share sum_r B_mr S_r with S_r = scaling * sum_k A_rk x_k.  Its error:
+
+* S: a sum of K products in fp32, off by at most K units of 2^-24 of the sum of their sizes, however it is ordered (for the
+  tensor cores K / 16 additions of 2^-22, the same number); times the scaling, one unit; for prompts rounded to bf16, 2^-8
+  of its size;
+* B S: rank products (exact in fp32) added to a sum that already holds the base: on the tensor cores rank / 16 + 1
+  additions off by at most 2^-22 each of the largest size the sum can have; by fp32 arithmetic (decoding) rank + 2
+  additions by 2^-23 each.
 """
 import ctypes
 
@@ -55,6 +59,25 @@ def share64(X, A, B, index, scaling):
             size[rows] = S.abs() @ B[a].abs().t()
             s_unit[rows] = (X[rows].abs() @ A[a].abs().t() * sc[a].abs()) @ B[a].abs().t()
     return out, s_unit, size
+
+
+def check_base(base, X, W, signs=None, scale=None):
+    """base (tokens, M): the fp32 result without adapters."""
+    K = X.shape[1]
+    x, w = X.double().cpu(), W.double().cpu()
+    if signs is not None:
+        x = x * signs.double().cpu()
+    h, n = x.clone(), 1
+    while n < K:
+        h = h.reshape(-1, K // (2 * n), 2, n)
+        h = torch.stack([h[:, :, 0] + h[:, :, 1], h[:, :, 0] - h[:, :, 1]], 2).reshape(-1, K)
+        n *= 2
+    h = h * (K ** -0.5 if scale is None else scale)
+    size = h.abs() @ w.abs().t()
+    logk = K.bit_length() - 1
+    allowed = size * 2.0 ** -8 + (logk + 1) * U * h.norm(dim=1)[:, None] * w.abs().sum(1)[None] * 1.01 + K / 16 * 2.0 ** -22 * size
+    off = (base.double().cpu() - h @ w.t()).abs()
+    assert bool((off <= allowed).all()), f"off by {float((off - allowed).max()):.3g} too much"
 
 
 def check_share(got, base, X, A, B, index, scaling, tensor_cores=True):
@@ -134,7 +157,7 @@ def test_c_entries_refuse_before_the_gpu(lib):
     assert gemv(N=0) == -2 and gemv(N=65) == -2
     assert l.b200ht_lora_gemm_workspace_bytes(48, 20, 128, 16) >= 20 * 128 * 2 + 20 * 16 * 2
     assert l.b200ht_lora_gemm_workspace_bytes(48, 0, 128, 16) == 0
-    assert l.b200ht_lora_gemv_workspace_bytes(48, 20, 16) >= (48 * 20 + 20 * 16) * 4
+    assert l.b200ht_lora_gemv_workspace_bytes(48, 128, 20, 16) >= (48 * 20 + 20 * 16) * 4
 
 
 # --------------------------------------------------------------------------------------------------------- on the GPU
@@ -153,13 +176,14 @@ SHAPES = [
 def test_prompts(pkg, shape, spread, layout):
     N, K, M, R, L = shape
     X, W, A, B, index, scaling = make(N, K, M, R, L, seed=N, spread=spread)
-    base = pkg.fused_ht_gemm(X, W, out_layout=layout)
+    base = pkg.lora_ht_gemm(X, W, A, B, torch.full_like(index, -1), out_layout=layout)
     got = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout=layout)
     half = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout=layout, out_dtype=torch.bfloat16)
     assert pkg.device_status() == 0
     assert torch.equal(half, got.bfloat16())   # the same sums, rounded once
     if layout == "mn":
         base, got = base.t(), got.t()
+    check_base(base, X, W)
     check_share(got, base, X, A, B, index, scaling)
 
 
@@ -167,7 +191,7 @@ def test_prompts(pkg, shape, spread, layout):
 @pytest.mark.parametrize("index", ["-1", "0", "2", "7"])
 def test_one_adapter_or_none_for_all(pkg, index):
     X, W, A, B, index, _ = make(400, 512, 200, 16, 3, spread=index)
-    base = pkg.fused_ht_gemm(X, W, out_layout="nm")
+    base = pkg.lora_ht_gemm(X, W, A, B, torch.full_like(index, -1), out_layout="nm")
     check_share(pkg.lora_ht_gemm(X, W, A, B, index, out_layout="nm"), base, X, A, B, index, None)
 
 
@@ -177,9 +201,10 @@ def test_split_launches_and_chunks(pkg, N, K, M, L):
     """The contraction in two launches (160 tiles of 256 rows on 148 SMs), and tokens in chunks that keep their transform in
     L2: tables, low-rank vectors and rows of B have to move along."""
     X, W, A, B, index, scaling = make(N, K, M, 16, L, seed=5)
-    base = pkg.fused_ht_gemm(X, W, out_layout="nm")
+    base = pkg.lora_ht_gemm(X, W, A, B, torch.full_like(index, -1), out_layout="nm")
     got = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, out_layout="nm")
     assert pkg.device_status() == 0
+    check_base(base, X, W)
     check_share(got, base, X, A, B, index, scaling)
 
 
@@ -187,7 +212,8 @@ def test_split_launches_and_chunks(pkg, N, K, M, L):
 def test_signs_and_scale_belong_to_the_transform(pkg):
     X, W, A, B, index, scaling = make(270, 512, 140, 32, 4, seed=6)
     signs = torch.randint(0, 2, (512,), generator=torch.Generator().manual_seed(1)).cuda() * 2 - 1
-    base = pkg.fused_ht_gemm(X, W, signs=signs, scale=0.5, out_layout="nm")
+    base = pkg.lora_ht_gemm(X, W, A, B, torch.full_like(index, -1), signs=signs, scale=0.5, out_layout="nm")
+    check_base(base, X, W, signs, 0.5)
     got = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, signs=signs, scale=0.5, out_layout="nm")
     check_share(got, base, X, A, B, index, scaling)
 
@@ -206,11 +232,15 @@ def test_decoding(pkg, shape, spread):
     columns, N, M, R, L = shape
     X, W, A, B, index, scaling = make(columns, N, M, R, L, seed=columns, spread=spread)
     Xc = X.t().contiguous()
-    base = pkg.fused_ht_gemv(W, Xc)
+    base = pkg.lora_ht_gemv(W, Xc, A, B, torch.full_like(index, -1))
     got = pkg.lora_ht_gemv(W, Xc, A, B, index, scaling=scaling)
     half = pkg.lora_ht_gemv(W, Xc, A, B, index, scaling=scaling, out_dtype=torch.bfloat16)
     assert pkg.device_status() == 0
     assert torch.equal(half, got.bfloat16())
+    if 256 <= N <= 8192:   # beyond, the base is fused_ht_gemv's own (tested with it)
+        check_base(base.t(), X, W)
+    else:
+        assert torch.equal(base, pkg.fused_ht_gemv(W, Xc))
     check_share(got.t(), base.t(), X, A, B, index, scaling, tensor_cores=False)
 
 
@@ -220,7 +250,7 @@ def test_decoding_beyond_one_pass_over_the_weight(pkg, columns):
     X, W, A, B, index, scaling = make(columns, 4096, 100, 16, 6, seed=8, spread="any")
     got = pkg.lora_ht_gemv(W, X.t().contiguous(), A, B, index, scaling=scaling)
     assert got.shape == (100, columns)
-    check_share(got.t(), pkg.fused_ht_gemm(X, W, out_layout="nm"), X, A, B, index, scaling)
+    check_share(got.t(), pkg.lora_ht_gemm(X, W, A, B, torch.full_like(index, -1), out_layout="nm"), X, A, B, index, scaling)
 
 
 @pytest.mark.gpu
@@ -320,7 +350,7 @@ def test_writes_stay_in_the_result_and_the_workspace(pkg, lib):
         for z in (ws[:guard], ws[guard + n:], C[:guard], C[guard + M * N * 2:]):
             assert bool((z == 0xA5).all())
         if N <= 64:
-            n = l.b200ht_lora_gemv_workspace_bytes(M, N, R)
+            n = l.b200ht_lora_gemv_workspace_bytes(M, K, N, R)
             ws = torch.full((n + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda")
             C.fill_(0xA5)
             Xc = X.t().contiguous()
