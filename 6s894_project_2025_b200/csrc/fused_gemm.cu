@@ -16,7 +16,10 @@ namespace b200ht {
 int launch_fwht_f32_split(const float *in, __nv_bfloat16 *split, uint64_t rows, uint32_t n, float scale, cudaStream_t st);
 int launch_fwht(const void *in, void *out, uint64_t rows, uint32_t n, int dtype, float scale, const void *signs,
                 cudaStream_t st, int keep_out = 0);
-int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, cudaStream_t st);
+int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, bool early, cudaStream_t st);
+int lora_gemm_split(int M, int N, int K);
+int launch_lora_gemm_split(const void *Y, const void *W, void *C, int M, int N, int K, int out_dtype, int out_layout, int split,
+                           const LoraGemm &lora, cudaStream_t st);
 int launch_gemm_bf16_tcgen05(const void *Y, const void *W, void *C, int M, int N, int K, int out_dtype,
                              int out_layout, cudaStream_t st, const float *row_scale = nullptr,
                              const float *tok_scale = nullptr, size_t ldc = 0, const LoraGemm *lora = nullptr);
@@ -251,9 +254,12 @@ static int fused_gemm_bf16(const void *X, const void *W, void *C, int M, int N, 
     }();
     const size_t row_bytes = (size_t)K * 2;
     if (chunk_bytes == 0 || K < 64 || (size_t)N * row_bytes <= chunk_bytes + chunk_bytes / 2) {
-        int rc = lora ? launch_lora_transform(X, workspace, N, K, scale, signs, st)
+        int rc = lora ? launch_lora_transform(X, workspace, N, K, scale, signs, true, st)
                       : launch_fwht(X, workspace, (uint64_t)N, (uint32_t)K, B200HT_BF16, scale, signs, st, 1);
         if (rc) return rc;
+        if (lora)
+            if (const int split = lora_gemm_split(M, N, K); split > 1)
+                return launch_lora_gemm_split(workspace, W, C, M, N, K, out_dtype, out_layout, split, *lora, st);
         return launch_gemm_bf16_tcgen05(workspace, W, C, M, N, K, out_dtype, out_layout, st, row_scale, tok_scale, 0,
                                         lora);
     }
@@ -265,7 +271,7 @@ static int fused_gemm_bf16(const void *X, const void *W, void *C, int M, int N, 
     for (long t0 = 0; t0 < N; t0 += per) {
         const int nt = (int)((N - t0) < per ? (N - t0) : per);
         const unsigned char *Xc = (const unsigned char *)X + (size_t)t0 * row_bytes;
-        int rc = lora ? launch_lora_transform(Xc, workspace, nt, K, scale, signs, st)
+        int rc = lora ? launch_lora_transform(Xc, workspace, nt, K, scale, signs, t0 == 0, st)
                       : launch_fwht(Xc, workspace, (uint64_t)nt, (uint32_t)K, B200HT_BF16, scale, signs, st, 1);
         if (rc) return rc;
         unsigned char *Cc = (unsigned char *)C + (out_layout == B200HT_OUT_MN ? (size_t)t0 : (size_t)t0 * M) * out_esz;

@@ -26,7 +26,7 @@
 #include <mutex>
 
 #include "tc_common.cuh"
-#include "lora.cuh"
+#include "lora_tc.cuh"
 
 namespace b200ht {
 
@@ -142,48 +142,7 @@ __device__ __forceinline__ void tc_tile_coord(int tile, int mt, int nt, TileOrde
 template <bool ADAPT>
 struct AdaptArgs {};
 template <>
-struct AdaptArgs<true> {
-    CUtensorMap tmB;     // [adapter][M][rank]
-    CUtensorMap tmS;     // [token][rank]
-    const int *tiles;    // kLoraTileInts a 256-token tile: number of its adapters, their numbers, ...
-    const int *index;    // adapter of each token
-    int adapters, rank;
-    int row;             // row of B of this launch's first row of C
-};
-
-// Groups of 16 tokens (bit g: tokens 16 g .. 16 g + 15 of the 256 x 64 tile at `tile`) that have a token of `adapter`.
-// In these groups the rows (128 bytes each) of tokens with another adapter are set to zero; those of tokens without one
-// are zero already.  `ids`: adapters of tokens lane, lane + 32, ... (negative: none).  One warp.
-__device__ __forceinline__ uint32_t tc_adapter_groups(uint32_t tile, const int (&ids)[TC_BN / 32], int adapter, int lane)
-{
-    uint32_t groups = 0, zeroed = 0;
-#pragma unroll
-    for (int i = 0; i < TC_BN / 32; ++i) {
-        const uint32_t own = __ballot_sync(0xffffffffu, ids[i] == adapter);
-        const uint32_t other = __ballot_sync(0xffffffffu, ids[i] >= 0 && ids[i] != adapter);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t bits = 0xffffu << (16 * h);
-            if (!(own & bits)) continue;
-            groups |= 1u << (2 * i + h);
-            if (!(other & bits)) continue;
-            zeroed = 1;
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {   // four rows an instruction
-                const int row = 16 * h + r + (lane >> 3);
-                if ((other >> row) & 1u)
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(tile + (uint32_t)((i * 32 + row) * 128 + (lane & 7) * 16)),
-                                 "r"(0)
-                                 : "memory");
-            }
-        }
-    }
-    if (zeroed) {
-        fence_proxy_async();
-        __syncwarp();
-    }
-    return groups;
-}
+struct AdaptArgs<true> : LoraOperands {};
 
 template <int OUT_DT, int LAYOUT, int MT, bool ADAPT>
 __global__ void __launch_bounds__(TcCfg<MT>::THREADS, 1)
@@ -315,14 +274,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 if constexpr (ADAPT) {
                     int mb, nb;
                     tc_tile_coord(tile, mt, nt, ord, mb, nb);
-                    const int *mine = adapt.tiles + (size_t)nb * kLoraTileInts;
-                    count = __ldcg(mine);
-#pragma unroll
-                    for (int i = 0; i < TC_BN / 32; ++i) {
-                        const int n = nb * TC_BN + i * 32 + lane;
-                        ids[i] = n < N ? __ldcg(adapt.index + n) : -1;
-                        list[i] = __ldcg(mine + 1 + i * 32 + lane);
-                    }
+                    count = lora_tile_tables(adapt, nb, N, lane, ids, list);
                 }
                 if (lane == 0) {
                     ok = mbar_wait(tempty_bar(acc), aph ^ 1u, abort_flag, status);
@@ -351,32 +303,19 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                     for (int i = 0; i < TC_BN / 32; ++i)
                         if (ids[i] >= adapt.adapters) ids[i] = -1;
                     for (int i = 0; i < count && ok; ++i) {
-                        int entry = list[0];
-#pragma unroll
-                        for (int j = 1; j < TC_BN / 32; ++j) entry = i >> 5 == j ? list[j] : entry;
-                        const int adapter = __shfl_sync(0xffffffffu, entry, i & 31);
+                        const int adapter = lora_list_entry(list, i);
                         for (int r = 0; r < adapt.rank; r += TC_BK, ++it) {
                             const int s = it % STAGES;
                             const uint32_t ph = (it / STAGES) & 1u;
                             ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, abort_flag, status));
                             if (!ok) break;
                             const uint32_t sa = base + s * STAGE_BYTES;
-                            uint32_t groups = tc_adapter_groups(sa + Cfg::A_BYTES, ids, adapter, lane);
+                            const uint32_t groups = tc_adapter_groups(sa + Cfg::A_BYTES, ids, adapter, lane);
                             if (lane == 0) {
                                 tc_fence_after();
-                                const int ksteps = adapt.rank - r >= TC_BK ? TC_BK / 16 : (adapt.rank - r + 15) / 16;
-                                while (groups) {   // one stretch of neighbouring groups after the other
-                                    const int g0 = __ffs(groups) - 1, n = __ffs(~(groups >> g0)) - 1;
-                                    groups &= ~(((1u << n) - 1) << g0);
-                                    const uint64_t bdesc = umma_desc_k_sw128(sa + Cfg::A_BYTES + g0 * 2048);
-                                    const uint32_t part = umma_idesc_bf16(128, 16 * n);
 #pragma unroll
-                                    for (int h = 0; h < MT; ++h) {
-                                        const uint64_t adesc = umma_desc_k_sw128(sa + h * 16384);
-                                        for (int k = 0; k < ksteps; ++k)
-                                            umma_bf16_ss(d_tmem + h * TC_BN + 16 * g0, adesc + 2 * k, bdesc + 2 * k, part, 1u);
-                                    }
-                                }
+                                for (int h = 0; h < MT; ++h)
+                                    lora_mma_groups(d_tmem + h * TC_BN, sa + h * 16384, sa + Cfg::A_BYTES, groups, adapt.rank - r);
                                 umma_commit(empty_bar(s));
                             }
                             __syncwarp();
@@ -663,8 +602,6 @@ int encode_tmap_bf16_row_groups(CUtensorMap *map, const void *base, uint64_t gro
     });
 }
 
-// [d2][d1][d0] bf16, d0 contiguous (d0 a multiple of 8), box 1 x box1 x 64 with 128-byte swizzle; a box that reaches
-// beyond d0 or d1 is filled with zeros.
 int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1)
 {
     EncodeTiledFn fn = get_encode_fn();
@@ -677,6 +614,20 @@ int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+// The operands of a contraction with adapters: B in boxes of `rows` rows, S of `tokens` tokens in boxes of `box` tokens.
+int lora_operands(LoraOperands *o, const LoraGemm &lora, int tokens, int rows, int box)
+{
+    int rc = encode_tmap_bf16_stack(&o->tmB, lora.B, (uint64_t)lora.adapters, (uint64_t)lora.M, (uint64_t)lora.rank, (uint32_t)rows);
+    if (rc) return rc;
+    rc = encode_tmap_bf16_stack(&o->tmS, lora.S, 1, (uint64_t)tokens, (uint64_t)lora.rank, (uint32_t)box);
+    o->tiles = lora.tiles;
+    o->index = lora.index;
+    o->adapters = lora.adapters;
+    o->rank = lora.rank;
+    o->row = lora.row;
+    return rc;
 }
 
 // Output map for the TMA-store epilogue: rows x cols of fp32 or bf16, box = 32 rows x 128 bytes, 128-byte swizzle.
@@ -719,15 +670,8 @@ static int launch_tc_mt(const void *Y, const void *W, void *C, int M, int N, int
     const int grid = tiles < sm_count() ? tiles : sm_count();
     if (lora) {
         AdaptArgs<true> ad{};
-        rc = encode_tmap_bf16_stack(&ad.tmB, lora->B, (uint64_t)lora->adapters, (uint64_t)lora->M, (uint64_t)lora->rank, Cfg::BM);
+        rc = lora_operands(&ad, *lora, N, Cfg::BM, TC_BN);
         if (rc) return rc;
-        rc = encode_tmap_bf16_stack(&ad.tmS, lora->S, 1, (uint64_t)N, (uint64_t)lora->rank, TC_BN);
-        if (rc) return rc;
-        ad.tiles = lora->tiles;
-        ad.index = lora->index;
-        ad.adapters = lora->adapters;
-        ad.rank = lora->rank;
-        ad.row = lora->row;
         rc = ensure_dyn_smem((const void *)gemm_tc_kernel<OUT_DT, LAYOUT, MT, true>, Cfg::SMEM_BYTES);
         if (rc) return rc;
         return launch_pdl(gemm_tc_kernel<OUT_DT, LAYOUT, MT, true>, dim3(grid), dim3(Cfg::THREADS), (size_t)Cfg::SMEM_BYTES, st,

@@ -12,26 +12,17 @@
 //                         lora_expand_kernel adds B S and rounds
 // Sums are fp32; S is rounded to bf16 where it becomes an operand of the tensor cores (like H(X) itself), and stays fp32
 // when decoding.  There is no counterpart in the reference.
-#include "lora.cuh"
-#include "tc_common.cuh"
+#include "lora_tc.cuh"
 
 namespace b200ht {
 
 int launch_fwht(const void *in, void *out, uint64_t rows, uint32_t n, int dtype, float scale, const void *signs,
                 cudaStream_t st, int keep_out);
-int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1);
 int launch_gemv_adapt(const void *W, const void *Xt, void *Y, int M, int N, int B, int out_dtype, const GemvAdapt &adapt,
                       cudaStream_t st);
 bool gemv_adapt_shape(int N, int B);
 int fused_gemm_bf16_lora(const void *X, const void *W, void *C, int M, int N, int K, int out_dtype, int out_layout, float scale,
                          const void *signs, void *workspace, cudaStream_t st, const LoraGemm &lora);
-
-// All threads of all CTAs of the cluster.
-__device__ __forceinline__ void cluster_sync_all()
-{
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
 
 // ---------------------------------------------------------------------------
 // Which adapters occur in each tile of tokens.  A token whose adapter no earlier token of the tile has opens its entry
@@ -42,8 +33,8 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
 {
     __shared__ __align__(16) int ids[256];
     __shared__ int opened[2][8];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();   // the rest of the chain starts after all earlier work: its kernels may read inputs at once
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long t = (long long)blockIdx.x * 256 + tid;
     int id = t < tokens ? index[t] : -1;
@@ -215,14 +206,17 @@ __device__ __forceinline__ void fwht_token(float *row, const __nv_bfloat16 *x, i
     else fwht_last<1>(row, out, K, scale);
 }
 
+// `early`: X is complete and Y free as soon as this kernel starts (it follows lora_plan_kernel); it then runs beside the
+// kernels in front and waits for them before it ends, so that whoever waits for it has waited for them too.
 __global__ void __launch_bounds__(512) lora_transform_kernel(const __nv_bfloat16 *X, __nv_bfloat16 *Y, int logk, float scale,
-                                                             const uint16_t *signs)
+                                                             const uint16_t *signs, int early)
 {
     extern __shared__ __align__(16) unsigned char smem_row[];
     pdl_launch_dependents();
-    pdl_wait();
+    if (!early) pdl_wait();
     const size_t at = (size_t)blockIdx.x << logk;
     fwht_token((float *)smem_row, X + at, 1, Y + at, logk, scale, signs);
+    if (early) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -562,27 +556,6 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-// launch_pdl with clusters of `cluster` CTAs along x.
-template <typename... KArgs, typename... Args>
-static int launch_pdl_cluster(void (*kernel)(KArgs...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args)
-{
-    note_launch();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-
 // Rows of A a block takes: one spreads a short call over the SMs; with enough tokens eight share the block's start.
 static int shrink_rows_of_block(int tokens, int rank)
 {
@@ -603,13 +576,13 @@ static int launch_shrink_rows(const void *X, const void *A, const int *index, co
                       (const __nv_bfloat16 *)X, stride, (const __nv_bfloat16 *)A, index, scaling, S, K, adapters, rank, rows);
 }
 
-int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, cudaStream_t st)
+int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, bool early, cudaStream_t st)
 {
     const int threads = K / 32 < 64 ? 64 : (K / 32 > 512 ? 512 : K / 32), smem = K * 4;
     int rc = ensure_dyn_smem((const void *)lora_transform_kernel, smem);
     if (rc) return rc;
     return launch_pdl(lora_transform_kernel, dim3((unsigned)tokens), dim3((unsigned)threads), (size_t)smem, st, (const __nv_bfloat16 *)X,
-                      (__nv_bfloat16 *)Y, ilog2((uint32_t)K), scale, (const uint16_t *)signs);
+                      (__nv_bfloat16 *)Y, ilog2((uint32_t)K), scale, (const uint16_t *)signs, early ? 1 : 0);
 }
 
 // Tokens from which the tile kernel serves a prompt (see launch_shrink_tiles).
