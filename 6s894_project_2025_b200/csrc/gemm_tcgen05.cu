@@ -270,11 +270,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 const int acc = tcount % NACC;
                 const uint32_t aph = (tcount / NACC) & 1u;
                 const uint32_t d_tmem = tmem_base + acc * TC_BN;   // MT == 2: halves at columns 0 and 256
-                int count = 0, ids[TC_BN / 32], list[TC_BN / 32];  // asked for ahead of the K loop: used behind it
+                LoraTileWalk walk{};   // asked for ahead of the K loop, used behind it
                 if constexpr (ADAPT) {
                     int mb, nb;
                     tc_tile_coord(tile, mt, nt, ord, mb, nb);
-                    count = lora_tile_tables(adapt, nb, N, lane, ids, list);
+                    walk.start(adapt.tiles + (size_t)nb * kLoraTileInts, 0, 1, lane);
                 }
                 if (lane == 0) {
                     ok = mbar_wait(tempty_bar(acc), aph ^ 1u, abort_flag, status);
@@ -299,18 +299,15 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                 if constexpr (ADAPT) {
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     it = __shfl_sync(0xffffffffu, it, 0);
-#pragma unroll
-                    for (int i = 0; i < TC_BN / 32; ++i)
-                        if (ids[i] >= adapt.adapters) ids[i] = -1;
-                    for (int i = 0; i < count && ok; ++i) {
-                        const int adapter = lora_list_entry(list, i);
+                    while (walk.more() && ok) {
+                        const uint32_t own = walk.next(lane);
                         for (int r = 0; r < adapt.rank; r += TC_BK, ++it) {
                             const int s = it % STAGES;
                             const uint32_t ph = (it / STAGES) & 1u;
                             ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, abort_flag, status));
                             if (!ok) break;
                             const uint32_t sa = base + s * STAGE_BYTES;
-                            const uint32_t groups = tc_adapter_groups(sa + Cfg::A_BYTES, ids, adapter, lane);
+                            const uint32_t groups = lora_groups(sa + Cfg::A_BYTES, own, walk.valid, lane);
                             if (lane == 0) {
                                 tc_fence_after();
 #pragma unroll
@@ -602,12 +599,13 @@ int encode_tmap_bf16_row_groups(CUtensorMap *map, const void *base, uint64_t gro
     });
 }
 
-int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1)
+int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1, uint64_t pitch)
 {
+    if (!pitch) pitch = d0;
     EncodeTiledFn fn = get_encode_fn();
     if (!fn) return (int)cudaErrorNotSupported;
     const cuuint64_t dims[3] = {d0, d1, d2};
-    const cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
+    const cuuint64_t strides[2] = {pitch * 2, pitch * d1 * 2};
     const cuuint32_t box[3] = {64, box1, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
@@ -621,10 +619,9 @@ int lora_operands(LoraOperands *o, const LoraGemm &lora, int tokens, int rows, i
 {
     int rc = encode_tmap_bf16_stack(&o->tmB, lora.B, (uint64_t)lora.adapters, (uint64_t)lora.M, (uint64_t)lora.rank, (uint32_t)rows);
     if (rc) return rc;
-    rc = encode_tmap_bf16_stack(&o->tmS, lora.S, 1, (uint64_t)tokens, (uint64_t)lora.rank, (uint32_t)box);
+    rc = encode_tmap_bf16_stack(&o->tmS, lora.S, 1, (uint64_t)tokens, (uint64_t)lora.rank, (uint32_t)box,
+                                (uint64_t)lora_pitch(lora.rank));
     o->tiles = lora.tiles;
-    o->index = lora.index;
-    o->adapters = lora.adapters;
     o->rank = lora.rank;
     o->row = lora.row;
     return rc;

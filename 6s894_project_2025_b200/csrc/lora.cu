@@ -12,6 +12,8 @@
 //                         lora_expand_kernel adds B S and rounds
 // Sums are fp32; S is rounded to bf16 where it becomes an operand of the tensor cores (like H(X) itself), and stays fp32
 // when decoding.  There is no counterpart in the reference.
+#include <type_traits>
+
 #include "lora_tc.cuh"
 
 namespace b200ht {
@@ -25,13 +27,15 @@ int fused_gemm_bf16_lora(const void *X, const void *W, void *C, int M, int N, in
                          const void *signs, void *workspace, cudaStream_t st, const LoraGemm &lora);
 
 // ---------------------------------------------------------------------------
-// Which adapters occur in each tile of tokens.  A token whose adapter no earlier token of the tile has opens its entry
-// in the list.  Earlier tokens of its warp are found by a match; only a warp's first token of an adapter looks through
-// the warps before, four tokens a load.
+// Which adapters occur in each tile of tokens, and where.  A token whose adapter no earlier token of the tile has opens
+// its entry in the list.  Earlier tokens of its warp are found by a match; only a warp's first token of an adapter looks
+// through the warps before, four tokens a load.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int tokens, int adapters, int *tiles)
 {
     __shared__ __align__(16) int ids[256];
+    __shared__ int entry[256];                 // entry of the adapter that this token opened
+    __shared__ unsigned own[256][8];           // tokens of each entry
     __shared__ int opened[2][8];
     pdl_wait();
     pdl_launch_dependents();   // the rest of the chain starts after all earlier work: its kernels may read inputs at once
@@ -40,45 +44,57 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
     int id = t < tokens ? index[t] : -1;
     if ((unsigned)id >= (unsigned)adapters) id = -1;
     ids[tid] = id;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) own[tid][w] = 0;
     const unsigned alike = __match_any_sync(0xffffffffu, id);   // by all lanes: not behind a condition
     const bool leads = id >= 0 && (alike & ((1u << lane) - 1)) == 0;
     __syncthreads();
-    bool before = false, before_half = false;   // an earlier warp has the adapter: of the tile, of its half
+    int earliest = tid;                        // first token of the tile with this adapter
+    bool before_half = false;                  // an earlier warp of this half has it
     if (leads) {
         const int4 *four = (const int4 *)ids;
         const int half0 = (warp & 4) * 8;
-#pragma unroll 8
-        for (int j = 0; j < warp * 8; ++j) {
+#pragma unroll 4
+        for (int j = warp * 8 - 1; j >= 0; --j) {
             const int4 v = four[j];
-            const bool hit = v.x == id || v.y == id || v.z == id || v.w == id;
-            before |= hit;
-            before_half |= hit && j >= half0;
+            if (v.w == id) earliest = 4 * j + 3;
+            if (v.z == id) earliest = 4 * j + 2;
+            if (v.y == id) earliest = 4 * j + 1;
+            if (v.x == id) earliest = 4 * j;
+            before_half |= j >= half0 && (v.x == id || v.y == id || v.z == id || v.w == id);
         }
     }
-    const bool first = leads && !before, first_half = leads && !before_half;
+    earliest = __shfl_sync(0xffffffffu, earliest, __ffs(alike) - 1);
+    const bool first = leads && earliest == tid, first_half = leads && !before_half;
     const unsigned b = __ballot_sync(0xffffffffu, first), bh = __ballot_sync(0xffffffffu, first_half);
+    const unsigned valid = __ballot_sync(0xffffffffu, id >= 0);
     if (lane == 0) {
         opened[0][warp] = __popc(b);
         opened[1][warp] = __popc(bh);
     }
     __syncthreads();
-    int at = __popc(b & ((1u << lane) - 1)), at_half = __popc(bh & ((1u << lane) - 1));
-    for (int w = 0; w < warp; ++w) at += opened[0][w];
-    for (int w = warp & 4; w < warp; ++w) at_half += opened[1][w];
+    int at = __popc(b & ((1u << lane) - 1)), at_half = __popc(bh & ((1u << lane) - 1)), n = 0, n_half = 0;
+    for (int w = 0; w < 8; ++w) {
+        if (w < warp) at += opened[0][w];
+        n += opened[0][w];
+        if ((w ^ warp) & 4) continue;
+        if (w < warp) at_half += opened[1][w];
+        n_half += opened[1][w];
+    }
     int *tile = tiles + (size_t)blockIdx.x * kLoraTileInts;
     int *half = tile + kLoraHalfOffset + (tid >> 7) * kLoraHalfInts;
-    if (first) tile[1 + at] = id;
+    if (first) {
+        tile[1 + at] = id;
+        entry[tid] = at;
+    }
     if (first_half) half[1 + at_half] = id;
-    if (tid == 0) {
-        int n = 0;
-        for (int w = 0; w < 8; ++w) n += opened[0][w];
-        tile[0] = n;
-    }
-    if ((tid & 127) == 0) {
-        int n = 0;
-        for (int w = warp; w < warp + 4; ++w) n += opened[1][w];
-        half[0] = n;
-    }
+    if (tid == 0) tile[0] = n;
+    if ((tid & 127) == 0) half[0] = n_half;
+    if (lane == 0) tile[kLoraValidOffset + warp] = (int)valid;
+    __syncthreads();
+    if (id >= 0) atomicOr(&own[entry[earliest]][warp], 1u << lane);
+    __syncthreads();
+    for (int i = tid; i < n * 8; i += 256) tile[kLoraOwnOffset + i] = (int)own[i >> 3][i & 7];
 }
 
 // ---------------------------------------------------------------------------
@@ -87,23 +103,25 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
 // error).  The row lies in shared memory as fp32 lines of 32 values, their 16-byte pieces exchanged by the line's number
 // so that no access below meets bank conflicts:
 //   A  32 consecutive values a thread from global memory: bits 0 .. 4 of the index
-//   B  rounds of up to five bits from bit 5 on, lanes side by side
-//   C  8 consecutive values and the last two bits: scaled, rounded, stored as 16-byte vectors
-// `stride`: distance of two elements of the token.
+//   B  rounds of up to five bits from bit 5 on, lanes side by side (one for K = 8192, two beyond)
+//   C  8 consecutive values and the last three bits: scaled, rounded, stored as 16-byte vectors
+// Bound: HBM, then shared memory (16 bytes an element and round).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int line_at(int e)   // place of element e
 {
     const int line = e >> 5;
     return (line << 5) | ((((e >> 2) ^ line) & 7) << 2) | (e & 3);
 }
-template <int BITS>
-__device__ __forceinline__ void fwht_round(float *row, int K, int bit)   // bits bit .. bit + BITS - 1, bit >= 5
+// `bit` and the sizes are constants, so that the places of a thread's elements differ by constants: in the line's number
+// by multiples of 2^(bit - 5), which exchange pieces only in its low three bits.
+template <int BITS, int BIT, int K>
+__device__ __forceinline__ void fwht_round(float *row)   // bits BIT .. BIT + BITS - 1, BIT >= 5
 {
     for (int task = threadIdx.x; task < (K >> BITS); task += blockDim.x) {
-        const int e0 = ((task >> bit) << (bit + BITS)) | (task & ((1 << bit) - 1));
+        const int at = line_at(((task >> BIT) << (BIT + BITS)) | (task & ((1 << BIT) - 1)));
         float v[1 << BITS];
 #pragma unroll
-        for (int i = 0; i < (1 << BITS); ++i) v[i] = row[line_at(e0 + (i << bit))];
+        for (int i = 0; i < (1 << BITS); ++i) v[i] = row[(at ^ (((i << (BIT - 5)) & 7) << 2)) + (i << BIT)];
 #pragma unroll
         for (int m = 1; m < (1 << BITS); m <<= 1)
 #pragma unroll
@@ -114,24 +132,25 @@ __device__ __forceinline__ void fwht_round(float *row, int K, int bit)   // bits
                     v[i | m] = a - b;
                 }
 #pragma unroll
-        for (int i = 0; i < (1 << BITS); ++i) row[line_at(e0 + (i << bit))] = v[i];
+        for (int i = 0; i < (1 << BITS); ++i) row[(at ^ (((i << (BIT - 5)) & 7) << 2)) + (i << BIT)] = v[i];
     }
     __syncthreads();
 }
-template <int BITS>
-__device__ __forceinline__ void fwht_last(const float *row, __nv_bfloat16 *out, int K, float scale)
+template <int BITS, int K>
+__device__ __forceinline__ void fwht_last(const float *row, __nv_bfloat16 *out, float scale)
 {
-    constexpr int N = 1 << BITS;
-    const int step = K >> BITS;
-    for (int task = threadIdx.x; task < step / 8; task += blockDim.x) {
+    constexpr int N = 1 << BITS, STEP = K >> BITS;
+    for (int task = threadIdx.x; task < STEP / 8; task += blockDim.x) {
         float v[N][8];
+        const int at0 = line_at(task * 8), at1 = line_at(task * 8 + 4);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float4 f = *(const float4 *)(row + line_at(task * 8 + i * step + 4 * h));
-                v[i][4 * h] = f.x, v[i][4 * h + 1] = f.y, v[i][4 * h + 2] = f.z, v[i][4 * h + 3] = f.w;
-            }
+        for (int i = 0; i < N; ++i) {
+            constexpr int LINES = STEP / 32;   // from one of the N pieces to the next
+            const int x = ((i * LINES) & 7) << 2;
+            const float4 f = *(const float4 *)(row + (LINES % 8 ? line_at(task * 8 + i * STEP) : (at0 ^ x) + i * STEP));
+            const float4 g = *(const float4 *)(row + (LINES % 8 ? line_at(task * 8 + i * STEP + 4) : (at1 ^ x) + i * STEP));
+            v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w, v[i][4] = g.x, v[i][5] = g.y, v[i][6] = g.z, v[i][7] = g.w;
+        }
 #pragma unroll
         for (int m = 1; m < N; m <<= 1)
 #pragma unroll
@@ -145,37 +164,32 @@ __device__ __forceinline__ void fwht_last(const float *row, __nv_bfloat16 *out, 
                     }
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            *(uint4 *)(out + task * 8 + i * step) =
+            *(uint4 *)(out + task * 8 + i * STEP) =
                 make_uint4(pack2<B200HT_BF16>(v[i][0] * scale, v[i][1] * scale), pack2<B200HT_BF16>(v[i][2] * scale, v[i][3] * scale),
                            pack2<B200HT_BF16>(v[i][4] * scale, v[i][5] * scale), pack2<B200HT_BF16>(v[i][6] * scale, v[i][7] * scale));
     }
 }
-// K = 2^logk >= 64; x: the token's first element; out: K values; signs: 0x8000 where an element is negated, or NULL.
-__device__ __forceinline__ void fwht_token(float *row, const __nv_bfloat16 *x, int stride, __nv_bfloat16 *out, int logk, float scale,
-                                           const uint16_t *signs)
+// K = 2^LOGK >= 64; x: the token's values, contiguous; out: K values; signs: 0x8000 where an element is negated, or NULL.
+template <int LOGK>
+__device__ __forceinline__ void fwht_token(float *row, const __nv_bfloat16 *x, __nv_bfloat16 *out, float scale, const uint16_t *signs)
 {
-    const int K = 1 << logk;
+    constexpr int K = 1 << LOGK, LAST = LOGK - 5 < 3 ? LOGK - 5 : 3, MIDDLE = LOGK - 5 - LAST;
     for (int task = threadIdx.x; task < K / 32; task += blockDim.x) {
         float v[32];
-        if (stride == 1) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 p = ((const uint4 *)(x + task * 32))[i];
-                if (signs) {
-                    const uint4 sg = ((const uint4 *)(signs + task * 32))[i];
-                    p.x ^= sg.x, p.y ^= sg.y, p.z ^= sg.z, p.w ^= sg.w;
-                }
-                const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = unpack2<B200HT_BF16>(w[e]);
-                    v[8 * i + 2 * e] = f.x;
-                    v[8 * i + 2 * e + 1] = f.y;
-                }
+        for (int i = 0; i < 4; ++i) {
+            uint4 p = ((const uint4 *)(x + task * 32))[i];
+            if (signs) {
+                const uint4 sg = ((const uint4 *)(signs + task * 32))[i];
+                p.x ^= sg.x, p.y ^= sg.y, p.z ^= sg.z, p.w ^= sg.w;
             }
-        } else {
+            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __bfloat162float(x[(size_t)(task * 32 + i) * stride]);
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<B200HT_BF16>(w[e]);
+                v[8 * i + 2 * e] = f.x;
+                v[8 * i + 2 * e + 1] = f.y;
+            }
         }
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1)
@@ -191,31 +205,34 @@ __device__ __forceinline__ void fwht_token(float *row, const __nv_bfloat16 *x, i
             *(float4 *)(row + line_at(task * 32 + 4 * i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     }
     __syncthreads();
-    const int last = logk >= 7 ? 2 : 1;
-    for (int bit = 5, left = logk - 5 - last; left > 0;) {
-        const int n = left <= 5 ? left : (left + 1) / 2;
-        if (n == 1) fwht_round<1>(row, K, bit);
-        else if (n == 2) fwht_round<2>(row, K, bit);
-        else if (n == 3) fwht_round<3>(row, K, bit);
-        else if (n == 4) fwht_round<4>(row, K, bit);
-        else fwht_round<5>(row, K, bit);
-        bit += n;
-        left -= n;
+    if constexpr (MIDDLE > 5) {
+        fwht_round<(MIDDLE + 1) / 2, 5, K>(row);
+        fwht_round<MIDDLE / 2, 5 + (MIDDLE + 1) / 2, K>(row);
+    } else if constexpr (MIDDLE > 0) {
+        fwht_round<MIDDLE, 5, K>(row);
     }
-    if (last == 2) fwht_last<2>(row, out, K, scale);
-    else fwht_last<1>(row, out, K, scale);
+    fwht_last<LAST, K>(row, out, scale);
+}
+// f(std::integral_constant<int, logk>) for logk = FROM .. 15.
+template <int FROM, typename F>
+static int with_logk(int logk, F f)
+{
+    if (logk == FROM) return f(std::integral_constant<int, FROM>{});
+    if constexpr (FROM < kMaxLogN) return with_logk<FROM + 1>(logk, f);
+    return B200HT_ERR_SIZE;
 }
 
 // `early`: X is complete and Y free as soon as this kernel starts (it follows lora_plan_kernel); it then runs beside the
 // kernels in front and waits for them before it ends, so that whoever waits for it has waited for them too.
-__global__ void __launch_bounds__(512) lora_transform_kernel(const __nv_bfloat16 *X, __nv_bfloat16 *Y, int logk, float scale,
-                                                             const uint16_t *signs, int early)
+template <int LOGK>
+__global__ void __launch_bounds__(256) lora_transform_kernel(const __nv_bfloat16 *X, __nv_bfloat16 *Y, float scale, const uint16_t *signs,
+                                                             int early)
 {
     extern __shared__ __align__(16) unsigned char smem_row[];
     pdl_launch_dependents();
     if (!early) pdl_wait();
-    const size_t at = (size_t)blockIdx.x << logk;
-    fwht_token((float *)smem_row, X + at, 1, Y + at, logk, scale, signs);
+    const size_t at = (size_t)blockIdx.x << LOGK;
+    fwht_token<LOGK>((float *)smem_row, X + at, Y + at, scale, signs);
     if (early) pdl_wait();
 }
 
@@ -275,8 +292,8 @@ lora_shrink_rows_kernel(const __nv_bfloat16 *X, int stride, const __nv_bfloat16 
     pdl_launch_dependents();
     pdl_wait();
     const int t = blockIdx.x, a = index[t];
-    shrink_rows<OUT>(X, stride, (size_t)t * (stride == 1 ? K : 1), A, a, (unsigned)a < (unsigned)adapters, scaling, S + (size_t)t * rank,
-                     (__nv_bfloat16 *)smem_row, K, rank, blockIdx.y * rows, rows);
+    shrink_rows<OUT>(X, stride, (size_t)t * (stride == 1 ? K : 1), A, a, (unsigned)a < (unsigned)adapters, scaling,
+                     S + (size_t)t * (sizeof(OUT) == 2 ? lora_pitch(rank) : rank), (__nv_bfloat16 *)smem_row, K, rank, blockIdx.y * rows, rows);
 }
 
 // Decoding: H(X) and S of every column in one launch.  It lets the next kernel start only once it has itself seen all
@@ -286,18 +303,18 @@ lora_shrink_rows_kernel(const __nv_bfloat16 *X, int stride, const __nv_bfloat16 
 // Several columns: a cluster of eight CTAs a column.  The elements of a column lie a row of X apart, a 32-byte sector
 // each, so every CTA fetches an eighth and they exchange it through distributed shared memory (each fetching all of it,
 // 272 CTAs of a batch of 16 at N = 4096 moved 35 MB through L2 and took 8 us).  Rank 0 transforms, the others divide A.
-template <bool CLUSTER>
+template <bool CLUSTER, int LOGK>
 __global__ void __launch_bounds__(256)
 lora_front_kernel(const __nv_bfloat16 *X, const __nv_bfloat16 *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S,
-                  int columns, int logk, float scale, int adapters, int rank, int rows)
+                  int columns, float scale, int adapters, int rank, int rows)
 {
     extern __shared__ __align__(16) unsigned char smem_row[];
     pdl_wait();
     pdl_launch_dependents();
-    const int K = 1 << logk;
+    constexpr int K = 1 << LOGK;
     if constexpr (!CLUSTER) {
         if (blockIdx.x == 0) {
-            fwht_token((float *)smem_row, X, 1, Xt, logk, scale, nullptr);
+            fwht_token<LOGK>((float *)smem_row, X, Xt, scale, nullptr);
         } else {
             const int a = index[0];
             shrink_rows<float>(X, 1, 0, A, a, (unsigned)a < (unsigned)adapters, scaling, S, nullptr, K, rank, (blockIdx.x - 1) * rows, rows);
@@ -322,7 +339,7 @@ lora_front_kernel(const __nv_bfloat16 *X, const __nv_bfloat16 *A, const int *ind
     }
     cluster_sync_all();   // no CTA writes again what others read, and none has left before they have
     if (part == 0) {
-        fwht_token((float *)(smem_row + K * 2), xs, 1, Xt + ((size_t)column << logk), logk, scale, nullptr);
+        fwht_token<LOGK>((float *)(smem_row + K * 2), xs, Xt + ((size_t)column << LOGK), scale, nullptr);
     } else {
         const int per = (rank + 6) / 7, r0 = (part - 1) * per, r1 = r0 + per < rank ? r0 + per : rank;
         const bool some = (unsigned)a < (unsigned)adapters;
@@ -465,7 +482,7 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
         for (int i = tid; i < rows * (rank / 8); i += kShrinkThreads) {
             const int t = t0 + row0 + i / (rank / 8);
             if (t < tokens && (unsigned)ids[t - t0] >= (unsigned)adapters)
-                *(uint4 *)(S + (size_t)t * rank + i % (rank / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+                *(uint4 *)(S + (size_t)t * lora_pitch(rank) + i % (rank / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
         }
 
     uint32_t it = 0, passes = 0;
@@ -540,7 +557,7 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
 #pragma unroll
             for (int p = 0; p < 8; ++p)
                 if (p < split) sum += v[p];
-            S[(size_t)(t0 + row) * rank + r] = __float2bfloat16_rn(sum * factor[row]);
+            S[(size_t)(t0 + row) * lora_pitch(rank) + r] = __float2bfloat16_rn(sum * factor[row]);
         }
         fence_proxy_async();   // the next pass' copies overwrite what was read here
         cluster_sync_all();
@@ -578,11 +595,14 @@ static int launch_shrink_rows(const void *X, const void *A, const int *index, co
 
 int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, bool early, cudaStream_t st)
 {
-    const int threads = K / 32 < 64 ? 64 : (K / 32 > 512 ? 512 : K / 32), smem = K * 4;
-    int rc = ensure_dyn_smem((const void *)lora_transform_kernel, smem);
-    if (rc) return rc;
-    return launch_pdl(lora_transform_kernel, dim3((unsigned)tokens), dim3((unsigned)threads), (size_t)smem, st, (const __nv_bfloat16 *)X,
-                      (__nv_bfloat16 *)Y, ilog2((uint32_t)K), scale, (const uint16_t *)signs, early ? 1 : 0);
+    const int threads = K / 64 < 64 ? 64 : (K / 64 > 256 ? 256 : K / 64), smem = K * 4;
+    return with_logk<6>(ilog2((uint32_t)K), [&](auto logk) {
+        const auto kernel = lora_transform_kernel<decltype(logk)::value>;
+        int rc = ensure_dyn_smem((const void *)kernel, smem);
+        if (rc) return rc;
+        return launch_pdl(kernel, dim3((unsigned)tokens), dim3((unsigned)threads), (size_t)smem, st, (const __nv_bfloat16 *)X,
+                          (__nv_bfloat16 *)Y, scale, (const uint16_t *)signs, early ? 1 : 0);
+    });
 }
 
 // Tokens from which the tile kernel serves a prompt (see launch_shrink_tiles).
@@ -615,22 +635,24 @@ static int launch_shrink_tiles(const void *X, const void *A, const int *index, c
 static int launch_front(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S, int columns,
                         int N, float scale, int adapters, int rank, cudaStream_t st)
 {
-    const int logk = ilog2((uint32_t)N);
-    if (columns == 1) {
-        const int rows = shrink_rows_of_block(1, rank), smem = N * 4;
-        int rc = ensure_dyn_smem((const void *)lora_front_kernel<false>, smem);
+    return with_logk<8>(ilog2((uint32_t)N), [&](auto logk) {
+        constexpr int LOGK = decltype(logk)::value < 14 ? decltype(logk)::value : 13;   // the streaming GEMV ends at 8192
+        if (columns == 1) {
+            const int rows = shrink_rows_of_block(1, rank), smem = N * 4;
+            int rc = ensure_dyn_smem((const void *)lora_front_kernel<false, LOGK>, smem);
+            if (rc) return rc;
+            return launch_pdl(lora_front_kernel<false, LOGK>, dim3((unsigned)(1 + (rank + rows - 1) / rows)), dim3(256), (size_t)smem, st,
+                              (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, 1, scale, adapters, rank, rows);
+        }
+        int rows = 1;   // rows of A at a time, of the seventh that a CTA has
+        while (rows < 8 && rows < (rank + 6) / 7) rows *= 2;
+        const int smem = N * 2 + N * 4;
+        int rc = ensure_dyn_smem((const void *)lora_front_kernel<true, LOGK>, smem);
         if (rc) return rc;
-        return launch_pdl(lora_front_kernel<false>, dim3((unsigned)(1 + (rank + rows - 1) / rows)), dim3(256), (size_t)smem, st,
-                          (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, 1, logk, scale, adapters, rank, rows);
-    }
-    int rows = 1;   // rows of A at a time, of the seventh that a CTA has
-    while (rows < 8 && rows < (rank + 6) / 7) rows *= 2;
-    const int smem = N * 2 + N * 4;
-    int rc = ensure_dyn_smem((const void *)lora_front_kernel<true>, smem);
-    if (rc) return rc;
-    return launch_pdl_cluster(lora_front_kernel<true>, 8, dim3((unsigned)columns * 8), dim3(256), (size_t)smem, st,
-                              (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, columns, logk, scale, adapters,
-                              rank, rows);
+        return launch_pdl_cluster(lora_front_kernel<true, LOGK>, 8, dim3((unsigned)columns * 8), dim3(256), (size_t)smem, st,
+                                  (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, columns, scale, adapters, rank,
+                                  rows);
+    });
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -650,7 +672,7 @@ extern "C" size_t b200ht_lora_gemm_workspace_bytes(int M, int N, int K, int rank
 {
     using namespace b200ht;
     if (M <= 0 || N <= 0 || K <= 0 || rank <= 0) return 0;
-    return b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16) + up256((size_t)N * rank * 2) +
+    return b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16) + up256((size_t)N * lora_pitch(rank) * 2) +
            up256(((size_t)N + 255) / 256 * kLoraTileInts * sizeof(int));
 }
 
@@ -674,14 +696,14 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     cudaStream_t st = (cudaStream_t)stream;
     unsigned char *ws = (unsigned char *)workspace + b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16);
     __nv_bfloat16 *S = (__nv_bfloat16 *)ws;
-    int *tiles = (int *)(ws + up256((size_t)N * rank * 2));
+    int *tiles = (int *)(ws + up256((size_t)N * lora_pitch(rank) * 2));
     const unsigned ntiles = (unsigned)((N + 255L) / 256);
     rc = launch_pdl(lora_plan_kernel, dim3(ntiles), dim3(256), 0, st, index, N, adapters, tiles);
     if (rc) return rc;
     rc = N >= kShrinkTileMin ? launch_shrink_tiles(X, A, index, scaling, tiles, S, N, K, adapters, rank, st)
                              : launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, 1, st);
     if (rc) return rc;
-    const LoraGemm lora{B, S, tiles, index, adapters, M, rank, 0};
+    const LoraGemm lora{B, S, tiles, adapters, M, rank, 0};
     return fused_gemm_bf16_lora(X, W, C, M, N, K, out_dtype, out_layout, scale, signs, workspace, st, lora);
 }
 

@@ -5,17 +5,24 @@
 namespace b200ht {
 
 constexpr int kLoraMaxRank = 128;
-// Table of one 256-token tile, made by lora_plan_kernel: the number of adapters among its tokens and their numbers, then
-// the same for each of its 128-token halves, each list in the order of first appearance.
+// Table of one 256-token tile, made by lora_plan_kernel: the number of adapters among its tokens and their numbers, in
+// the order of first appearance; the same for each of its 128-token halves; 256 bits: tokens with an adapter; 256 bits for
+// each adapter of the list: its tokens.
 constexpr int kLoraHalfOffset = 257, kLoraHalfInts = 129;
-constexpr int kLoraTileInts = 516;   // 1 + 256 + 2 * (1 + 128), to a multiple of four
+constexpr int kLoraValidOffset = kLoraHalfOffset + 2 * kLoraHalfInts, kLoraOwnOffset = kLoraValidOffset + 8;
+constexpr int kLoraTileInts = kLoraOwnOffset + 256 * 8 + 1;   // a multiple of four
+static_assert(kLoraTileInts % 4 == 0, "tables of tiles keep their alignment");
+
+// Elements from one token's low-rank vector to the next: whole lines of 128 bytes, so that the copies of a tile by all CTAs
+// at once spread over the L2 (256 tokens of rank 16 side by side are 64 lines; 128 CTAs fetching them for 16 adapters each
+// took 15 us longer than with a line a token).
+constexpr int lora_pitch(int rank) { return (rank + 63) & ~63; }
 
 // The adapters of one contraction, as its launcher takes them.
 struct LoraGemm {
     const void *B;       // [adapters][M][rank] bf16
-    const void *S;       // [tokens][rank] bf16: scaling * A x of each token's adapter, 0 without one
+    const void *S;       // [tokens][lora_pitch(rank)] bf16, rank of each used: scaling * A x of each token's adapter, 0 without one
     const int *tiles;    // kLoraTileInts per 256-token tile
-    const int *index;    // adapter of each token
     int adapters, M, rank;
     int row;             // row of B that belongs to the first row of C
 
@@ -24,9 +31,8 @@ struct LoraGemm {
     {
         LoraGemm o = *this;
         o.row += (int)r;
-        o.S = (const unsigned char *)S + (size_t)t * rank * 2;
+        o.S = (const unsigned char *)S + (size_t)t * lora_pitch(rank) * 2;
         o.tiles = tiles + (size_t)(t / 256) * kLoraTileInts;
-        o.index = index + t;
         return o;
     }
 };

@@ -70,7 +70,9 @@ lora_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
         if (lane == 0) {
             const int *tile = lora.tiles + (size_t)nb * kLoraTileInts;
             const int count = __ldcg(tile);
-            int it = 0;
+            int it = 0, queue[4];   // this CTA's next adapters
+#pragma unroll
+            for (int i = 0; i < 4; ++i) queue[i] = __ldcg(tile + 1 + part + i * split);   // entries up to 31: in the table
             for (; it < nk; ++it) {
                 const int s = it % stages;
                 const uint32_t sa = base + s * stage_bytes;
@@ -81,9 +83,10 @@ lora_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
                 }
                 tma_load_2d(sa + 16384, &tmY, (kb0 + it) * 64, n0, full_bar(s));
             }
-            int adapter = part < count ? __ldcg(tile + 1 + part) : 0;
             for (int i = part; i < count && ok; i += split) {
-                const int next = i + split < count ? __ldcg(tile + 1 + i + split) : 0;
+                const int adapter = queue[0];
+                queue[0] = queue[1], queue[1] = queue[2], queue[2] = queue[3];
+                if (i + 4 * split < count) queue[3] = __ldcg(tile + 1 + i + 4 * split);
                 for (int r = 0; r < lora.rank; r += 64, ++it) {
                     const int s = it % stages;
                     if (!mbar_wait(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, status)) { ok = false; break; }
@@ -91,7 +94,6 @@ lora_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
                     tma_load_3d(base + s * stage_bytes, &lora.tmB, r, lora.row + m0, adapter, full_bar(s));
                     tma_load_3d(base + s * stage_bytes + 16384, &lora.tmS, r, n0, 0, full_bar(s));
                 }
-                adapter = next;
             }
             if (!ok) {   // copies on their way still land in this CTA's shared memory: give them time
                 const int pending = it < stages ? it : stages;
@@ -102,8 +104,8 @@ lora_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
             }
         }
     } else if (warp == 1) {
-        int ids[kLoraTile / 32], list[kLoraTile / 32];
-        const int count = lora_tile_tables(lora, nb, N, lane, ids, list);
+        LoraTileWalk walk;
+        walk.start(lora.tiles + (size_t)nb * kLoraTileInts, part, split, lane);
         const uint32_t idesc = umma_idesc_bf16(128, box);
         int it = 0;
         if (lane == 0)
@@ -119,17 +121,14 @@ lora_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
             }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         it = nk;
-#pragma unroll
-        for (int i = 0; i < kLoraTile / 32; ++i)
-            if (ids[i] >= lora.adapters) ids[i] = -1;
-        for (int i = part; i < count && ok; i += split) {
-            const int adapter = lora_list_entry(list, i);
+        while (walk.more() && ok) {
+            const uint32_t own = walk.next(lane);
             for (int r = 0; r < lora.rank; r += 64, ++it) {
                 const int s = it % stages;
                 ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (it / stages) & 1u, abort_flag, status));
                 if (!ok) break;
                 const uint32_t sa = base + s * stage_bytes;
-                const uint32_t groups = tc_adapter_groups(sa + 16384, ids, adapter, lane);
+                const uint32_t groups = lora_groups(sa + 16384, own, walk.valid, lane);
                 if (lane == 0) {
                     tc_fence_after();
                     lora_mma_groups(tmem, sa, sa + 16384, groups, lora.rank - r);

@@ -12,70 +12,91 @@ struct LoraOperands {
     CUtensorMap tmB;     // [adapter][M][rank]
     CUtensorMap tmS;     // [token][rank]
     const int *tiles;    // kLoraTileInts a 256-token tile: number of its adapters, their numbers, ...
-    const int *index;    // adapter of each token
-    int adapters, rank;
+    int rank;
     int row;             // row of B of this launch's first row of C
 };
 
-// Host: [d2][d1][d0] bf16, d0 contiguous (a multiple of 8), boxes of 1 x box1 x 64 with 128-byte swizzle; a box that
-// reaches beyond d0 or d1 is filled with zeros.
-int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1);
+// Host: [d2][d1][d0] bf16, rows of d0 contiguous values `pitch` apart (a multiple of 8; 0: d0), boxes of 1 x box1 x 64 with
+// 128-byte swizzle; a box that reaches beyond d0 or d1 is filled with zeros.
+int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint64_t d1, uint64_t d0, uint32_t box1,
+                           uint64_t pitch = 0);
 int lora_operands(LoraOperands *o, const LoraGemm &lora, int tokens, int rows, int box);
 
-// Groups of 16 tokens (bit g: tokens 16 g .. 16 g + 15 of the tile of 128-byte rows at `tile`) that have a token of `adapter`.
-// In these groups the rows (128 bytes each) of tokens with another adapter are set to zero; those of tokens without one
-// are zero already.  `ids`: adapters of tokens lane, lane + 32, ... (negative: none).  One warp.
-__device__ __forceinline__ uint32_t tc_adapter_groups(uint32_t tile, const int (&ids)[kLoraTile / 32], int adapter, int lane)
+// One warp's walk over entries first, first + step, ... of a tile's list: lane w < 8 gets word w of the tokens with an
+// adapter, and of those of the entry's.  Four entries a load, the next four under way.
+struct LoraTileWalk {
+    const int *tile;
+    int count, at, step;      // entries of the list; the next one to hand out
+    uint32_t valid, now, ahead;
+
+    __device__ __forceinline__ uint32_t fetch(int entry, int lane) const
+    {
+        entry += (lane >> 3) * step;
+        return entry < count ? (uint32_t)__ldcg(tile + kLoraOwnOffset + entry * 8 + (lane & 7)) : 0u;
+    }
+    __device__ __forceinline__ void start(const int *t, int first, int by, int lane)
+    {
+        tile = t;
+        at = first;
+        step = by;
+        valid = lane < 8 ? (uint32_t)__ldcg(t + kLoraValidOffset + lane) : 0u;
+        count = __ldcg(t);
+        // before the count is known: all 256 entries have their place in the table
+        now = (uint32_t)__ldcg(t + kLoraOwnOffset + min(first + (lane >> 3) * by, 255) * 8 + (lane & 7));
+        ahead = 0;
+        taken = 0;
+    }
+    __device__ __forceinline__ bool more() const { return at < count; }
+    __device__ __forceinline__ uint32_t next(int lane)   // by the whole warp
+    {
+        if (taken == 0) ahead = fetch(at + 4 * step, lane);
+        const uint32_t word = __shfl_sync(0xffffffffu, now, taken * 8 + (lane & 7));
+        at += step;
+        if (++taken == 4) {
+            taken = 0;
+            now = ahead;
+        }
+        return lane < 8 ? word : 0u;
+    }
+    int taken;                // of the four
+};
+
+// Bit i of the low eight at bit 2 i.
+__device__ __forceinline__ uint32_t spread_bits(uint32_t x)
 {
-    uint32_t groups = 0, zeroed = 0;
-#pragma unroll
-    for (int i = 0; i < kLoraTile / 32; ++i) {
-        const uint32_t own = __ballot_sync(0xffffffffu, ids[i] == adapter);
-        const uint32_t other = __ballot_sync(0xffffffffu, ids[i] >= 0 && ids[i] != adapter);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t bits = 0xffffu << (16 * h);
-            if (!(own & bits)) continue;
-            groups |= 1u << (2 * i + h);
-            if (!(other & bits)) continue;
-            zeroed = 1;
+    x = (x | (x << 4)) & 0x0f0fu;
+    x = (x | (x << 2)) & 0x3333u;
+    return (x | (x << 1)) & 0x5555u;
+}
+
+// Groups of 16 tokens (bit g: tokens 16 g .. 16 g + 15 of the tile of 128-byte rows at `rows`) that have a token of `own`.
+// In these groups the rows of tokens with another adapter are set to zero; those of tokens without one are zero already.
+// By one warp.  Short code rather than unrolled: it runs a few times a tile and costs most by being fetched.
+__device__ __forceinline__ uint32_t lora_groups(uint32_t rows, uint32_t own, uint32_t valid, int lane)
+{
+    const uint32_t other = valid & ~own;
+    const bool lo = own & 0xffffu, hi = own >> 16;
+    const uint32_t groups = spread_bits(__ballot_sync(0xffffffffu, lo)) | (spread_bits(__ballot_sync(0xffffffffu, hi)) << 1);
+    uint32_t mixed = spread_bits(__ballot_sync(0xffffffffu, lo && (other & 0xffffu))) |
+                     (spread_bits(__ballot_sync(0xffffffffu, hi && (other >> 16))) << 1);
+    if (mixed) {
+#pragma unroll 1
+        for (; mixed; mixed &= mixed - 1) {
+            const int g = __ffs(mixed) - 1;
+            const uint32_t bits = __shfl_sync(0xffffffffu, other, g >> 1) >> (16 * (g & 1));
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {   // four rows an instruction
-                const int row = 16 * h + r + (lane >> 3);
-                if ((other >> row) & 1u)
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(tile + (uint32_t)((i * 32 + row) * 128 + (lane & 7) * 16)),
+                const int row = r + (lane >> 3);
+                if ((bits >> row) & 1u)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(rows + (uint32_t)((g * 16 + row) * 128 + (lane & 7) * 16)),
                                  "r"(0)
                                  : "memory");
             }
         }
-    }
-    if (zeroed) {
         fence_proxy_async();
         __syncwarp();
     }
     return groups;
-}
-
-// One warp's view of tile `nb`: adapters of tokens lane, lane + 32, ..., the list of the tile's adapters the same way.
-// Returns their number.  (Numbers from `adapters` on are no adapters: the caller drops them once the loads have arrived.)
-__device__ __forceinline__ int lora_tile_tables(const LoraOperands &o, int nb, int tokens, int lane, int (&ids)[kLoraTile / 32],
-                                                int (&list)[kLoraTile / 32])
-{
-    const int *tile = o.tiles + (size_t)nb * kLoraTileInts;
-#pragma unroll
-    for (int i = 0; i < kLoraTile / 32; ++i) {
-        const int n = nb * kLoraTile + i * 32 + lane;
-        ids[i] = n < tokens ? __ldcg(o.index + n) : -1;
-        list[i] = __ldcg(tile + 1 + i * 32 + lane);
-    }
-    return __ldcg(tile);
-}
-__device__ __forceinline__ int lora_list_entry(const int (&list)[kLoraTile / 32], int i)   // by the whole warp
-{
-    int entry = list[0];
-#pragma unroll
-    for (int j = 1; j < kLoraTile / 32; ++j) entry = i >> 5 == j ? list[j] : entry;
-    return __shfl_sync(0xffffffffu, entry, i & 31);
 }
 
 // D[:, tokens of `groups`] += B . S^T for 128 rows of B at `b` and the tokens at `s`: one instruction for each stretch of
