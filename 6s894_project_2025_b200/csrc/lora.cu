@@ -5,7 +5,7 @@
 //
 //   H(X)                  lora_transform_kernel: fp32 throughout, one rounding to bf16
 //   S = s_a * A_a x_t     lora_shrink_rows_kernel (few tokens: a block per token and some rows of A) or
-//                         lora_shrink_tile_kernel (tcgen05: 128 tokens against the adapters among them)
+//                         lora_shrink_tile_kernel (tcgen05: 256 tokens against the adapters among them)
 //   C = W . H(X) + B S    prompts: further K steps of the contraction itself (gemm_tcgen05.cu), one rounding;
 //                         decoding: lora_front_kernel (H(X) and S in one launch), then the streaming GEMV, which adds
 //                         B S to its sums (fused_gemv.cu); shapes that do not take it: fused GEMV into fp32, then
@@ -27,33 +27,26 @@ int fused_gemm_bf16_lora(const void *X, const void *W, void *C, int M, int N, in
                          const void *signs, void *workspace, cudaStream_t st, const LoraGemm &lora);
 
 // ---------------------------------------------------------------------------
-// Which adapters occur in each tile of tokens, and where.  A token whose adapter no earlier token of the tile has opens
-// its entry in the list.  Earlier tokens of its warp are found by a match; only a warp's first token of an adapter looks
-// through the warps before, four tokens a load.
+// Which adapters occur among 256 tokens.  Called by 256 threads, eight warps, with the token's adapter (-1: none); a token
+// whose adapter no earlier one has opens an entry.  Earlier tokens of its warp are found by a match; only a warp's first
+// token of an adapter looks through the warps before, four tokens a load.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int tokens, int adapters, int *tiles)
+struct TileAdapters {
+    __align__(16) int ids[256];
+    int entry[256];      // entry of the adapter that this token opened
+    int opened[8];
+};
+// Returns the number of entries; `mine`: this token's, `first`: it opened it.  `sync` is a barrier of the 256 threads.
+template <typename Sync>
+__device__ __forceinline__ int tile_adapters(TileAdapters &t, int tid, int id, int &mine, bool &first, Sync sync)
 {
-    __shared__ __align__(16) int ids[256];
-    __shared__ int entry[256];                 // entry of the adapter that this token opened
-    __shared__ unsigned own[256][8];           // tokens of each entry
-    __shared__ int opened[2][8];
-    pdl_wait();
-    pdl_launch_dependents();   // the rest of the chain starts after all earlier work: its kernels may read inputs at once
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long t = (long long)blockIdx.x * 256 + tid;
-    int id = t < tokens ? index[t] : -1;
-    if ((unsigned)id >= (unsigned)adapters) id = -1;
-    ids[tid] = id;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) own[tid][w] = 0;
+    const int lane = tid & 31, warp = tid >> 5;
+    t.ids[tid] = id;
     const unsigned alike = __match_any_sync(0xffffffffu, id);   // by all lanes: not behind a condition
-    const bool leads = id >= 0 && (alike & ((1u << lane) - 1)) == 0;
-    __syncthreads();
-    int earliest = tid;                        // first token of the tile with this adapter
-    bool before_half = false;                  // an earlier warp of this half has it
-    if (leads) {
-        const int4 *four = (const int4 *)ids;
-        const int half0 = (warp & 4) * 8;
+    sync();
+    int earliest = tid;
+    if (id >= 0 && (alike & ((1u << lane) - 1)) == 0) {
+        const int4 *four = (const int4 *)t.ids;
 #pragma unroll 4
         for (int j = warp * 8 - 1; j >= 0; --j) {
             const int4 v = four[j];
@@ -61,38 +54,46 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
             if (v.z == id) earliest = 4 * j + 2;
             if (v.y == id) earliest = 4 * j + 1;
             if (v.x == id) earliest = 4 * j;
-            before_half |= j >= half0 && (v.x == id || v.y == id || v.z == id || v.w == id);
         }
     }
     earliest = __shfl_sync(0xffffffffu, earliest, __ffs(alike) - 1);
-    const bool first = leads && earliest == tid, first_half = leads && !before_half;
-    const unsigned b = __ballot_sync(0xffffffffu, first), bh = __ballot_sync(0xffffffffu, first_half);
-    const unsigned valid = __ballot_sync(0xffffffffu, id >= 0);
-    if (lane == 0) {
-        opened[0][warp] = __popc(b);
-        opened[1][warp] = __popc(bh);
-    }
-    __syncthreads();
-    int at = __popc(b & ((1u << lane) - 1)), at_half = __popc(bh & ((1u << lane) - 1)), n = 0, n_half = 0;
+    first = id >= 0 && earliest == tid;
+    const unsigned b = __ballot_sync(0xffffffffu, first);
+    if (lane == 0) t.opened[warp] = __popc(b);
+    sync();
+    int at = __popc(b & ((1u << lane) - 1)), n = 0;
     for (int w = 0; w < 8; ++w) {
-        if (w < warp) at += opened[0][w];
-        n += opened[0][w];
-        if ((w ^ warp) & 4) continue;
-        if (w < warp) at_half += opened[1][w];
-        n_half += opened[1][w];
+        if (w < warp) at += t.opened[w];
+        n += t.opened[w];
     }
+    if (first) t.entry[tid] = at;
+    sync();
+    mine = id >= 0 ? t.entry[earliest] : -1;
+    return n;
+}
+
+// The tables of the tiles (lora.cuh).
+__global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int tokens, int adapters, int *tiles)
+{
+    __shared__ TileAdapters found;
+    __shared__ unsigned own[256][8];
+    pdl_wait();
+    pdl_launch_dependents();   // the rest of the chain starts after all earlier work: its kernels may read inputs at once
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long t = (long long)blockIdx.x * 256 + tid;
+    int id = t < tokens ? index[t] : -1;
+    if ((unsigned)id >= (unsigned)adapters) id = -1;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) own[tid][w] = 0;
+    int mine;
+    bool first;
+    const int n = tile_adapters(found, tid, id, mine, first, [] { __syncthreads(); });
     int *tile = tiles + (size_t)blockIdx.x * kLoraTileInts;
-    int *half = tile + kLoraHalfOffset + (tid >> 7) * kLoraHalfInts;
-    if (first) {
-        tile[1 + at] = id;
-        entry[tid] = at;
-    }
-    if (first_half) half[1 + at_half] = id;
+    if (first) tile[1 + mine] = id;
     if (tid == 0) tile[0] = n;
-    if ((tid & 127) == 0) half[0] = n_half;
+    const unsigned valid = __ballot_sync(0xffffffffu, id >= 0);
     if (lane == 0) tile[kLoraValidOffset + warp] = (int)valid;
-    __syncthreads();
-    if (id >= 0) atomicOr(&own[entry[earliest]][warp], 1u << lane);
+    if (id >= 0) atomicOr(&own[mine][warp], 1u << lane);
     __syncthreads();
     for (int i = tid; i < n * 8; i += 256) tile[kLoraOwnOffset + i] = (int)own[i >> 3][i & 7];
 }
@@ -282,18 +283,20 @@ __device__ __forceinline__ void shrink_rows(const __nv_bfloat16 *X, int stride, 
     }
 }
 
-// stride: distance of two elements of a token; token t begins at t * (stride == 1 ? K : 1).
+// stride: distance of two elements of a token; token t begins at t * (stride == 1 ? K : 1).  `early`: as in
+// lora_transform_kernel.
 template <typename OUT>
 __global__ void __launch_bounds__(256)
 lora_shrink_rows_kernel(const __nv_bfloat16 *X, int stride, const __nv_bfloat16 *A, const int *index, const float *scaling, OUT *S,
-                        int K, int adapters, int rank, int rows)
+                        int K, int adapters, int rank, int rows, int early)
 {
     extern __shared__ __align__(16) unsigned char smem_row[];
     pdl_launch_dependents();
-    pdl_wait();
+    if (!early) pdl_wait();
     const int t = blockIdx.x, a = index[t];
     shrink_rows<OUT>(X, stride, (size_t)t * (stride == 1 ? K : 1), A, a, (unsigned)a < (unsigned)adapters, scaling,
                      S + (size_t)t * (sizeof(OUT) == 2 ? lora_pitch(rank) : rank), (__nv_bfloat16 *)smem_row, K, rank, blockIdx.y * rows, rows);
+    if (early) pdl_wait();
 }
 
 // Decoding: H(X) and S of every column in one launch.  It lets the next kernel start only once it has itself seen all
@@ -401,22 +404,24 @@ lora_expand_kernel(const float *base, const __nv_bfloat16 *B, const float *S, co
 }
 
 // ---------------------------------------------------------------------------
-// S of many tokens, on the tensor cores: the A matrices of 128 / rank adapters (the M of the instruction) against 128
-// tokens (N), K split over the CTAs of a cluster.  Each token keeps the rows of its own adapter; the tile's list of
-// adapters is walked in passes.  With prompts a tile has one or two adapters and X is read once; bound then: the bytes of
-// X.  (An instruction costs its issuer the same whatever its N, so the adapters share one; with the tokens as M and one
-// instruction an adapter, 16384 x 8192 tokens of 40 requests at rank 64 took 94 us.)
+// S of many tokens, on the tensor cores: 256 tokens (the N of the instruction) against the A matrices of the adapters among
+// them, 128 / rank of which share the M of one instruction, two such groups a pass; K is split over the CTAs of a cluster.
+// Each token keeps the rows of its own adapter.  With prompts a tile has a few adapters, one pass serves them and X is read
+// once; bound then: the bytes of X.  (An instruction takes about 90 ns whatever its M and N, so it should be full: with 128
+// tokens as M and an instruction an adapter, 16384 x 8192 tokens of 40 requests at rank 64 took 94 us; with the adapters as
+// M and 128 tokens as N, 97 us, two tiles an SM taking turns and a second pass where a tile had three adapters.)
 //
-// Warp 0 copies by TMA (X 128 x 64 and rank x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the MMAs,
-// warps 2..5 bring the accumulator (one row of an A a lane) into shared memory, over the stages that have been used up.
-// The CTAs of the cluster then add the partial sums of 128 / cluster tokens each through distributed shared memory, in
-// the order of the ranks, and write them with one rounding: no atomics, no partial sums in memory.
+// Warp 0 copies by TMA (X 256 x 64 and rank x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the MMAs,
+// warps 2..9 find the tile's adapters while the first tiles of X arrive, and at the end bring the accumulators (one row of
+// an A a lane) into shared memory, over the stages that have been used up.  The CTAs of the cluster then add the partial
+// sums of 256 / cluster tokens each through distributed shared memory, in the order of the ranks, and write them with one
+// rounding: no atomics, no partial sums in memory.
+// The kernel runs beside lora_plan_kernel (its inputs are complete when it starts) and waits for it at its end.
 // ---------------------------------------------------------------------------
-constexpr int kShrinkTokens = 128, kShrinkStages = 3, kShrinkThreads = 192, kShrinkColumns = 128;
-constexpr int kShrinkXBytes = kShrinkTokens * 128, kShrinkABytes = 128 * 128;
-constexpr int kShrinkStageBytes = kShrinkXBytes + kShrinkABytes;
+constexpr int kShrinkStages = 3, kShrinkThreads = 320;
+constexpr int kShrinkXBytes = 256 * 128, kShrinkStageBytes = 2 * kShrinkXBytes;
 constexpr int kShrinkSmem = kShrinkStages * kShrinkStageBytes + 1024 + 128;
-static_assert(kShrinkTokens * (kLoraMaxRank + 1) * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
+static_assert(256 * (kLoraMaxRank + 1) * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
 
 __device__ __forceinline__ float cluster_load(uint32_t local, int rank)   // the float at `local` in the shared memory of CTA `rank`
 {
@@ -426,14 +431,16 @@ __device__ __forceinline__ float cluster_load(uint32_t local, int rank)   // the
     asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
-__global__ void __launch_bounds__(kShrinkThreads, 2)
-lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const int *tiles,
-                        const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int adapters, int rank, int per_pass,
-                        int kblocks, int split, int *status)
+
+__global__ void __launch_bounds__(kShrinkThreads, 1)
+lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const int *index,
+                        const float *scaling, __nv_bfloat16 *S, int tokens, int adapters, int rank, int kblocks, int split, int *status)
 {
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ int ids[kShrinkTokens], list[kShrinkTokens];   // adapter of each token; the adapters of the tile
-    __shared__ float factor[kShrinkTokens];                   // scaling of each token's adapter
+    __shared__ TileAdapters found;
+    __shared__ int list[256], slot[256];   // the tile's adapters; each token's place among them
+    __shared__ float factor[256];          // scaling of each token's adapter
+    __shared__ int count_s;
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char *gen = smem_dyn + (base - smem_u32(smem_dyn));
     const uint32_t bars = base + kShrinkStages * kShrinkStageBytes;
@@ -443,12 +450,13 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
     uint32_t *tmem_slot = (uint32_t *)(gen + kShrinkStages * kShrinkStageBytes + 16 * kShrinkStages + 8);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int part = blockIdx.x % split, tile = blockIdx.x / split;   // rank in the cluster, 128-token tile
-    const int t0 = tile * kShrinkTokens;
+    const int part = blockIdx.x % split, tile = blockIdx.x / split;   // rank in the cluster, 256-token tile
+    const int t0 = tile * 256;
+    const int nk = kblocks / split, kb0 = part * nk, ahead = nk < kShrinkStages ? nk : kShrinkStages;
 
     if (tid == 0) {
         for (int s = 0; s < kShrinkStages; ++s) {
-            mbar_init(full_bar(s), 1);
+            mbar_init(full_bar(s), 2);   // X, the A matrices
             mbar_init(empty_bar(s), 1);
         }
         mbar_init(done_bar, 1);
@@ -457,99 +465,120 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
         tma_prefetch_desc(&tmX);
         tma_prefetch_desc(&tmA);
     }
-    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), kShrinkColumns);
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();   // not before this CTA has its TMEM: the contraction behind takes all of it
-    pdl_wait();
 
-    const int *table = tiles + (size_t)(tile >> 1) * kLoraTileInts + kLoraHalfOffset + (tile & 1) * kLoraHalfInts;
-    const int count = __ldcg(table);
-    if (tid < kShrinkTokens) {
-        const int id = t0 + tid < tokens ? __ldcg(index + t0 + tid) : -1;
-        ids[tid] = id;
-        factor[tid] = scaling && (unsigned)id < (unsigned)adapters ? scaling[id] : 1.f;
-        if (tid < count) list[tid] = __ldcg(table + 1 + tid);
+    auto load_x = [&](int s, int kb) {
+        mbar_expect_tx(full_bar(s), (uint32_t)kShrinkXBytes);
+        tma_load_3d(base + s * kShrinkStageBytes, &tmX, kb * 64, t0, 0, full_bar(s));
+    };
+    if (warp == 0) {
+        if (lane == 0)
+            for (int i = 0; i < ahead; ++i) load_x(i, kb0 + i);
+        __syncwarp();
+    } else if (warp >= 2) {
+        const int t = tid - 64;
+        int id = t0 + t < tokens ? __ldcg(index + t0 + t) : -1, mine;
+        if ((unsigned)id >= (unsigned)adapters) id = -1;
+        bool first;
+        factor[t] = scaling && id >= 0 ? scaling[id] : 1.f;
+        const int n = tile_adapters(found, t, id, mine, first, [] { asm volatile("bar.sync 1, 256;\n" ::: "memory"); });
+        slot[t] = mine;
+        if (first) list[mine] = id;
+        if (t == 0) count_s = n;
     }
     __syncthreads();
-    const int kb0 = kblocks / split * part, kb1 = kb0 + kblocks / split;
-    float *partial = (float *)gen;                  // [128][rank + 1], over the stages
-    const int pitch = rank + 1;
-    const int rows = kShrinkTokens / split, row0 = part * rows;   // tokens whose sums this CTA writes
+    const int count = count_s;
+    const int share = 128 / rank;                   // adapters of one instruction
+    float *partial = (float *)gen;                  // [256][rank + 1], over the stages
+    const int pitch = rank + 1, out_pitch = lora_pitch(rank);
+    const int rows = 256 / split, row0 = part * rows;   // tokens whose sums this CTA writes
     if (blockIdx.y == 0)                            // tokens without an adapter
         for (int i = tid; i < rows * (rank / 8); i += kShrinkThreads) {
-            const int t = t0 + row0 + i / (rank / 8);
-            if (t < tokens && (unsigned)ids[t - t0] >= (unsigned)adapters)
-                *(uint4 *)(S + (size_t)t * lora_pitch(rank) + i % (rank / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+            const int row = row0 + i / (rank / 8);
+            if (t0 + row < tokens && slot[row] < 0)
+                *(uint4 *)(S + (size_t)(t0 + row) * out_pitch + i % (rank / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
         }
 
-    uint32_t it = 0, passes = 0;
-    bool ok = true;   // once a wait has run out this CTA copies and multiplies no more, but keeps step with its cluster
-    for (int first = blockIdx.y * per_pass; first < count; first += gridDim.y * per_pass, ++passes) {
-        const int n = count - first < per_pass ? count - first : per_pass;
+    int it = 0, passes = 0;   // K steps so far; X of the first `ahead` is on its way
+    bool ok = true;           // once a wait has run out this CTA copies and multiplies no more, but keeps step with its cluster
+    for (int first = blockIdx.y * 2 * share; first < count; first += gridDim.y * 2 * share, ++passes) {
+        const int n = count - first < 2 * share ? count - first : 2 * share;   // adapters of this pass, `share` a group
+        const int groups = n > share ? 2 : 1;
         if (!ok) {
         } else if (warp == 0 && lane == 0) {
-            uint32_t i2 = it;
-            for (int kb = kb0; kb < kb1 && ok; ++kb, ++i2) {
+            int i2 = it;
+            for (int kb = kb0; kb < kb0 + nk; ++kb, ++i2) {
                 const int s = i2 % kShrinkStages;
-                if (!mbar_wait(empty_bar(s), ((i2 / kShrinkStages) & 1u) ^ 1u, abort_flag, status)) { ok = false; break; }
-                mbar_expect_tx(full_bar(s), (uint32_t)(kShrinkXBytes + n * rank * 128));
-                const uint32_t sa = base + s * kShrinkStageBytes;
-                tma_load_3d(sa, &tmX, kb * 64, t0, 0, full_bar(s));
-                for (int a = 0; a < n; ++a)
-                    tma_load_3d(sa + kShrinkXBytes + a * rank * 128, &tmA, kb * 64, 0, list[first + a], full_bar(s));
+                if (i2 >= ahead) {
+                    if (!mbar_wait(empty_bar(s), ((i2 / kShrinkStages) & 1u) ^ 1u, abort_flag, status)) { ok = false; break; }
+                    load_x(s, kb);
+                }
+                mbar_expect_tx(full_bar(s), (uint32_t)(n * rank * 128));
+                uint32_t to = base + s * kShrinkStageBytes + kShrinkXBytes;
+                for (int a = 0; a < n; ++a) {
+                    if (a == share) to = base + s * kShrinkStageBytes + kShrinkXBytes + 16384;
+                    tma_load_3d(to, &tmA, kb * 64, 0, list[first + a], full_bar(s));
+                    to += rank * 128;
+                }
             }
             if (!ok) {   // copies on their way still land in this CTA's shared memory: give them time
-                const uint32_t pending = i2 < (uint32_t)kShrinkStages ? i2 : (uint32_t)kShrinkStages;
-                for (uint32_t j = 1; j <= pending; ++j) {
+                const int pending = i2 < kShrinkStages ? i2 : kShrinkStages;
+                for (int j = 1; j <= pending; ++j) {
                     const uint64_t ns = global_ns();
                     while (!mbar_test(full_bar((i2 - j) % kShrinkStages), ((i2 - j) / kShrinkStages) & 1u) && global_ns() - ns < 100000000ull) {}
                 }
             }
         } else if (warp == 1 && lane == 0) {
-            constexpr uint32_t idesc = umma_idesc_bf16(128, kShrinkTokens);
-            uint32_t i2 = it;
-            for (int kb = kb0; kb < kb1; ++kb, ++i2) {
+            constexpr uint32_t idesc = umma_idesc_bf16(128, 256);
+            int i2 = it;
+            for (int kb = 0; kb < nk; ++kb, ++i2) {
                 const int s = i2 % kShrinkStages;
                 if (!mbar_wait(full_bar(s), (i2 / kShrinkStages) & 1u, abort_flag, status)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t sa = base + s * kShrinkStageBytes;
+                const uint64_t xdesc = umma_desc_k_sw128(sa);
                 // rows of the A operand behind the adapters' hold whatever was there: their sums are not read
-                const uint64_t xdesc = umma_desc_k_sw128(sa), adesc = umma_desc_k_sw128(sa + kShrinkXBytes);
+                for (int g = 0; g < groups; ++g) {
+                    const uint64_t adesc = umma_desc_k_sw128(sa + kShrinkXBytes + g * 16384);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_bf16_ss(tmem, adesc + 2 * k, xdesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem + g * 256, adesc + 2 * k, xdesc + 2 * k, idesc, (kb | k) ? 1u : 0u);
+                }
                 umma_commit(empty_bar(s));
             }
             if (ok) umma_commit(done_bar);
         }
         __syncwarp();
-        it += (uint32_t)(kb1 - kb0);
-        // all MMAs of the pass done: the accumulator is complete and the stages are free
+        it += nk;
+        // all MMAs of the pass done: the accumulators are complete and the stages are free
         ok = __syncthreads_and(ok && mbar_wait(done_bar, passes & 1u, abort_flag, status));
         if (ok && warp >= 2) {
             tc_fence_after();
             const int q = warp & 3, row = q * 32 + lane, a = row / rank, r = row - a * rank;
-            const int id = a < n ? list[first + a] : -1;   // -1 (no adapter) is no token's that is looked for here
+            const int c0 = (warp - 2) / 4 * 128;   // two warps share the lanes of a quadrant
 #pragma unroll 1
-            for (int c = 0; c < kShrinkTokens; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-                tmem_ld_wait();
+            for (int g = 0; g < groups; ++g) {
+                const int mine = a < share && g * share + a < n ? first + g * share + a : -2;   // -2 is no token's place
+#pragma unroll 1
+                for (int c = c0; c < c0 + 128; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + g * 256 + c, v);
+                    tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (a < n && ids[c + i] == id) partial[(c + i) * pitch + r] = __uint_as_float(v[i]);
+                    for (int i = 0; i < 32; ++i)
+                        if (slot[c + i] == mine) partial[(c + i) * pitch + r] = __uint_as_float(v[i]);
+                }
             }
             tc_fence_before();
         }
         cluster_sync_all();
         for (int i = tid; i < rows * rank && ok; i += kShrinkThreads) {
-            const int row = row0 + i / rank, r = i % rank, id = ids[row];
-            bool mine = false;
-            for (int a = 0; a < n; ++a) mine |= id == list[first + a];
-            if (!mine) continue;
+            const int row = row0 + i / rank, r = i % rank, mine = slot[row] - first;
+            if (mine < 0 || mine >= n) continue;
             const uint32_t at = base + (uint32_t)((row * pitch + r) * 4);
             float v[8], sum = 0.f;
 #pragma unroll
@@ -557,16 +586,22 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
 #pragma unroll
             for (int p = 0; p < 8; ++p)
                 if (p < split) sum += v[p];
-            S[(size_t)(t0 + row) * lora_pitch(rank) + r] = __float2bfloat16_rn(sum * factor[row]);
+            S[(size_t)(t0 + row) * out_pitch + r] = __float2bfloat16_rn(sum * factor[row]);
         }
         fence_proxy_async();   // the next pass' copies overwrite what was read here
         cluster_sync_all();
     }
+    if (passes == 0 && warp == 0 && lane == 0)   // nothing to do here, but X has been asked for: let it arrive
+        for (int i = 0; i < ahead; ++i) {
+            mbar_arrive(full_bar(i));
+            mbar_wait(full_bar(i), 0u, abort_flag, status);
+        }
+    pdl_wait();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, kShrinkColumns);
+        tmem_dealloc(tmem, 512);
     }
 }
 
@@ -583,14 +618,14 @@ static int shrink_rows_of_block(int tokens, int rank)
 
 template <typename OUT>
 static int launch_shrink_rows(const void *X, const void *A, const int *index, const float *scaling, OUT *S, int tokens, int K,
-                              int adapters, int rank, int stride, cudaStream_t st)
+                              int adapters, int rank, int stride, bool early, cudaStream_t st)
 {
     const int rows = shrink_rows_of_block(tokens, rank);
     const size_t smem = stride == 1 ? 0 : (size_t)K * 2;
     int rc = ensure_dyn_smem((const void *)lora_shrink_rows_kernel<OUT>, (int)smem);
     if (rc) return rc;
     return launch_pdl(lora_shrink_rows_kernel<OUT>, dim3((unsigned)tokens, (unsigned)((rank + rows - 1) / rows)), dim3(256), smem, st,
-                      (const __nv_bfloat16 *)X, stride, (const __nv_bfloat16 *)A, index, scaling, S, K, adapters, rank, rows);
+                      (const __nv_bfloat16 *)X, stride, (const __nv_bfloat16 *)A, index, scaling, S, K, adapters, rank, rows, early ? 1 : 0);
 }
 
 int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale, const void *signs, bool early, cudaStream_t st)
@@ -605,31 +640,32 @@ int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale
     });
 }
 
-// Tokens from which the tile kernel serves a prompt (see launch_shrink_tiles).
-constexpr int kShrinkTileMin = 65;
+// Few tokens: a block for each, which reads its A through L2 (5 TB/s or so, whatever the tokens' order); from 32 MB of such
+// reads on the tile kernel, which needs about 12 us for a few adapters a tile and 15 more for each further pass.  At 256
+// tokens, K = 4096, rank 16 (32 MB): 7 us against 13 (one adapter) and 29 (64 adapters).
+static bool shrink_by_rows(int tokens, int K, int rank) { return (size_t)tokens * rank * K * 2 <= (size_t)32 << 20; }
 
-static int launch_shrink_tiles(const void *X, const void *A, const int *index, const float *scaling, const int *tiles,
-                               __nv_bfloat16 *S, int tokens, int K, int adapters, int rank, cudaStream_t st)
+static int launch_shrink_tiles(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int K,
+                               int adapters, int rank, cudaStream_t st)
 {
-    const int per_pass = 128 / rank;
     CUtensorMap tx, ta;
-    int rc = encode_tmap_bf16_stack(&tx, X, 1, (uint64_t)tokens, (uint64_t)K, kShrinkTokens);
+    int rc = encode_tmap_bf16_stack(&tx, X, 1, (uint64_t)tokens, (uint64_t)K, 256);
     if (rc) return rc;
     rc = encode_tmap_bf16_stack(&ta, A, (uint64_t)adapters, (uint64_t)rank, (uint64_t)K, (uint32_t)rank);
     if (rc) return rc;
     rc = ensure_dyn_smem((const void *)lora_shrink_tile_kernel, kShrinkSmem);
     if (rc) return rc;
-    // K over a cluster of up to eight CTAs while all of them find room at once (two an SM), then the passes over the
-    // adapters of a tile over blockIdx.y the same way
-    const int ntiles = (tokens + kShrinkTokens - 1) / kShrinkTokens, room = 2 * sm_count();
+    // K over a cluster of up to eight CTAs while all of them find an SM at once, then the passes over the adapters of a
+    // tile over blockIdx.y the same way
+    const int ntiles = (tokens + 255) / 256, per_pass = 128 / rank * 2;
     int split = 1;
-    while (split < 8 && split * 2 <= K / 64 && ntiles * split * 2 <= room) split *= 2;
-    const int most = adapters < kShrinkTokens ? adapters : kShrinkTokens, passes = (most + per_pass - 1) / per_pass;
-    int ways = room / (ntiles * split);
+    while (split < 8 && split * 2 <= K / 64 && ntiles * split * 2 <= sm_count()) split *= 2;
+    const int most = adapters < 256 ? adapters : 256, passes = (most + per_pass - 1) / per_pass;
+    int ways = sm_count() / (ntiles * split);
     ways = ways < 1 ? 1 : (ways > passes ? passes : ways);
     return launch_pdl_cluster(lora_shrink_tile_kernel, (unsigned)split, dim3((unsigned)(ntiles * split), (unsigned)ways),
-                              dim3(kShrinkThreads), (size_t)kShrinkSmem, st, tx, ta, tiles, index, scaling, S, tokens, adapters, rank,
-                              per_pass, K / 64, split, status_word_ptr());
+                              dim3(kShrinkThreads), (size_t)kShrinkSmem, st, tx, ta, index, scaling, S, tokens, adapters, rank, K / 64,
+                              split, status_word_ptr());
 }
 
 static int launch_front(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S, int columns,
@@ -700,8 +736,8 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     const unsigned ntiles = (unsigned)((N + 255L) / 256);
     rc = launch_pdl(lora_plan_kernel, dim3(ntiles), dim3(256), 0, st, index, N, adapters, tiles);
     if (rc) return rc;
-    rc = N >= kShrinkTileMin ? launch_shrink_tiles(X, A, index, scaling, tiles, S, N, K, adapters, rank, st)
-                             : launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, 1, st);
+    rc = shrink_by_rows(N, K, rank) ? launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, 1, true, st)
+                                    : launch_shrink_tiles(X, A, index, scaling, S, N, K, adapters, rank, st);
     if (rc) return rc;
     const LoraGemm lora{B, S, tiles, adapters, M, rank, 0};
     return fused_gemm_bf16_lora(X, W, C, M, N, K, out_dtype, out_layout, scale, signs, workspace, st, lora);
@@ -741,7 +777,7 @@ extern "C" int b200ht_lora_gemv(const void *W, const void *X, void *Y, const voi
         return launch_gemv_adapt(W, Xt, Y, M, N, B, out_dtype, GemvAdapt{Bm, S, index, adapters, rank}, st);
     }
     float *base = (float *)workspace, *S = (float *)((unsigned char *)workspace + up256((size_t)M * B * sizeof(float)));
-    rc = launch_shrink_rows(X, A, index, scaling, S, B, N, adapters, rank, B, st);
+    rc = launch_shrink_rows(X, A, index, scaling, S, B, N, adapters, rank, B, false, st);
     if (rc) return rc;
     rc = b200ht_fused_gemv(W, X, base, M, N, B, B200HT_BF16, B200HT_F32, scale, stream);
     if (rc) return rc;

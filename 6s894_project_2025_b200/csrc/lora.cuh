@@ -6,12 +6,8 @@ namespace b200ht {
 
 constexpr int kLoraMaxRank = 128;
 // Table of one 256-token tile, made by lora_plan_kernel: the number of adapters among its tokens and their numbers, in
-// the order of first appearance; the same for each of its 128-token halves; 256 bits: tokens with an adapter; 256 bits for
-// each adapter of the list: its tokens.
-constexpr int kLoraHalfOffset = 257, kLoraHalfInts = 129;
-constexpr int kLoraValidOffset = kLoraHalfOffset + 2 * kLoraHalfInts, kLoraOwnOffset = kLoraValidOffset + 8;
-constexpr int kLoraTileInts = kLoraOwnOffset + 256 * 8 + 1;   // a multiple of four
-static_assert(kLoraTileInts % 4 == 0, "tables of tiles keep their alignment");
+// the order of first appearance; 256 bits: tokens with an adapter; 256 bits for each adapter of the list: its tokens.
+constexpr int kLoraValidOffset = 257, kLoraOwnOffset = kLoraValidOffset + 8, kLoraTileInts = kLoraOwnOffset + 256 * 8;
 
 // Elements from one token's low-rank vector to the next: whole lines of 128 bytes, so that the copies of a tile by all CTAs
 // at once spread over the L2 (256 tokens of rank 16 side by side are 64 lines; 128 CTAs fetching them for 16 adapters each

@@ -166,6 +166,8 @@ SHAPES = [
     (1, 64, 8, 8, 1), (1, 1024, 300, 16, 4), (3, 256, 130, 64, 5), (17, 512, 64, 24, 3), (64, 1024, 96, 128, 2),
     (65, 128, 200, 8, 40), (127, 512, 77, 32, 3), (129, 256, 256, 72, 6), (255, 64, 129, 16, 100), (256, 1024, 384, 64, 4),
     (257, 512, 1, 40, 2), (300, 2048, 130, 120, 9), (1000, 256, 520, 16, 7), (1537, 512, 250, 56, 30), (700, 4096, 64, 128, 3),
+    # enough reads of A for the tensor cores' kernel: one K step a CTA, several passes over the adapters, straddled groups
+    (1100, 4096, 40, 8, 90), (530, 8192, 72, 24, 25), (2100, 1024, 33, 72, 20), (70, 32768, 16, 120, 9), (9000, 256, 24, 40, 3),
 ]
 
 
