@@ -729,6 +729,10 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     if ((uintptr_t)workspace & 255u) return B200HT_ERR_ALIGN;
     rc = check_device();
     if (rc) return rc;
+    // one token: the layouts of both entries are the same, and the streaming GEMV is the faster form
+    if (N == 1 && !signs && gemv_adapt_shape(K, 1))
+        return b200ht_lora_gemv(W, X, C, A, B, index, scaling, M, K, 1, adapters, rank, out_dtype, scale, workspace, workspace_bytes,
+                                stream);
     cudaStream_t st = (cudaStream_t)stream;
     unsigned char *ws = (unsigned char *)workspace + b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16);
     __nv_bfloat16 *S = (__nv_bfloat16 *)ws;

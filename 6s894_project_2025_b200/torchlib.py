@@ -13,6 +13,8 @@ under the ``b200ht`` namespace:
   — autograd: the inverse call on the incoming gradients.
 * ``torch.ops.b200ht.norm_rotary_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, axis_order,
   interleaved, hadamard)`` — autograd: gradients of q, k and both weights.
+* ``torch.ops.b200ht.lora_ht_gemm(X, W, A, B, index, scaling, scale, token_major, out_bf16)`` and
+  ``torch.ops.b200ht.lora_ht_gemv(W, X, A, B, index, scaling, scale, out_bf16)`` — serving operators, no gradient.
 
 All run the CUDA library; there is no CPU kernel behind them.
 """
@@ -22,7 +24,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-from . import heads, ops
+from . import heads, lora, ops
 
 
 @torch.library.custom_op("b200ht::hadamard_transform", mutates_args=(), device_types="cuda")
@@ -152,3 +154,28 @@ def _norm_rotary_backward(ctx, dq, dk):
 
 
 norm_rotary_qk_op.register_autograd(_norm_rotary_backward, setup_context=_norm_rotary_setup)
+
+
+@torch.library.custom_op("b200ht::lora_ht_gemm", mutates_args=(), device_types="cuda")
+def lora_ht_gemm_op(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, index: torch.Tensor,
+                    scaling: Optional[torch.Tensor], scale: float, token_major: bool, out_bf16: bool) -> torch.Tensor:
+    return lora.lora_ht_gemm(X, W, A, B, index, scaling=scaling, scale=scale, out_layout="nm" if token_major else "mn",
+                             out_dtype=torch.bfloat16 if out_bf16 else torch.float32)
+
+
+@lora_ht_gemm_op.register_fake
+def _(X, W, A, B, index, scaling, scale, token_major, out_bf16):
+    n, m = X.shape[0], W.shape[0]
+    return X.new_empty((n, m) if token_major else (m, n), dtype=torch.bfloat16 if out_bf16 else torch.float32)
+
+
+@torch.library.custom_op("b200ht::lora_ht_gemv", mutates_args=(), device_types="cuda")
+def lora_ht_gemv_op(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Tensor, index: torch.Tensor,
+                    scaling: Optional[torch.Tensor], scale: float, out_bf16: bool) -> torch.Tensor:
+    return lora.lora_ht_gemv(W, X, A, B, index, scaling=scaling, scale=scale,
+                             out_dtype=torch.bfloat16 if out_bf16 else torch.float32)
+
+
+@lora_ht_gemv_op.register_fake
+def _(W, X, A, B, index, scaling, scale, out_bf16):
+    return W.new_empty((W.shape[0], X.shape[1] if X.dim() == 2 else 1), dtype=torch.bfloat16 if out_bf16 else torch.float32)

@@ -397,3 +397,41 @@ def test_projection_with_adapters_then_norm_and_rotation(pkg):
     q1, k1 = pkg.norm_rotary_qk(one[:, :hq], one[:, hq:hq + hk], qw, kw, pos[last], inv, hadamard=True)
     assert_close(q1, forward64(one[:, :hq], qw, 1e-6, pos[last], inv, hadamard=True))
     assert k1.shape == (8, hk, D)
+
+
+@pytest.mark.gpu
+def test_registered_operators(pkg):
+    X, W, A, B, index, scaling = make(300, 512, 96, 16, 4, seed=15)
+    Xc = X[:8].t().contiguous()
+    tests = ("test_schema", "test_faketensor")
+    torch.library.opcheck(torch.ops.b200ht.lora_ht_gemm, (X, W, A, B, index, scaling, 0.5, True, True), test_utils=tests)
+    torch.library.opcheck(torch.ops.b200ht.lora_ht_gemm, (X, W, A, B, index, None, 0.5, False, False), test_utils=tests)
+    torch.library.opcheck(torch.ops.b200ht.lora_ht_gemv, (W, Xc, A, B, index[:8], scaling, 0.5, False), test_utils=tests)
+    want = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling, scale=0.5, out_layout="nm", out_dtype=torch.bfloat16)
+    assert torch.equal(torch.ops.b200ht.lora_ht_gemm(X, W, A, B, index, scaling, 0.5, True, True), want)
+    with pytest.raises(RuntimeError):   # a serving operator: no gradient
+        torch.ops.b200ht.lora_ht_gemm(X.float().bfloat16().requires_grad_(), W, A, B, index, scaling, 0.5, True, False).sum().backward()
+
+
+@pytest.mark.gpu
+def test_another_stream_than_the_current_one_waits_its_turn(pkg):
+    """Inputs written on a side stream just before the call on it: every kernel of the chain starts after them."""
+    X, W, A, B, index, scaling = make(700, 2048, 512, 32, 9, seed=16, spread="any")
+    Xc = X[:8].t().contiguous()
+    want = pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling), pkg.lora_ht_gemv(W, Xc, A, B, index[:8], scaling=scaling)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(10):
+            late = [torch.zeros_like(t) for t in (X, W, A, B, index, scaling, Xc)]
+            busy = torch.randn(2048, 2048, device="cuda")
+            for _ in range(5):
+                busy = busy @ busy * 1e-3
+            for t, v in zip(late, (X, W, A, B, index, scaling, Xc)):
+                t.copy_(v)
+            x, w, a, b, i, sc, xc = late
+            got = pkg.lora_ht_gemm(x, w, a, b, i, scaling=sc), pkg.lora_ht_gemv(w, xc, a, b, i[:8], scaling=sc)
+            for t in late:      # and the inputs may be overwritten right behind the call
+                t.zero_()
+            assert all(torch.equal(u, v) for u, v in zip(got, want))
+    assert pkg.device_status() == 0
