@@ -704,7 +704,9 @@ gemv_bf16_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __nv_bflo
             const int row = grp_row0 + r;
             if (r < group_rows && row < row_end) {
                 if (ADAPT) sum += extra[(grp % extra_groups * group_rows + r) * Bg + c];
-                store_out(Y, (size_t)row * B + b0 + c, sum, out_dtype);
+                size_t at = (size_t)row * B + b0 + c;
+                if constexpr (ADAPT) at = row * adapt.a.y_row + (b0 + c) * adapt.a.y_column;
+                store_out(Y, at, sum, out_dtype);
                 // the same value, with the call's tag beside it, into the slot arrays of the other ranks: one 8-byte
                 // store each, which arrives whole, so a peer that reads the tag has the value
                 const size_t slot = (size_t)(po.row_begin + row) * B + c;

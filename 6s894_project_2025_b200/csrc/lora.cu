@@ -302,8 +302,9 @@ lora_shrink_rows_kernel(const __nv_bfloat16 *X, int stride, const __nv_bfloat16 
 // Decoding: H(X) and S of every column in one launch.  It lets the next kernel start only once it has itself seen all
 // earlier work complete, so the streaming GEMV behind it may read W, B and index at once and waits for nothing but Xt and S.
 //
-// One column (CLUSTER false): block 0 transforms, the others take `rows` rows of A each, x comes straight from memory.
-// Several columns: a cluster of eight CTAs a column.  The elements of a column lie a row of X apart, a 32-byte sector
+// Tokens whose elements lie side by side (CLUSTER false; a single column too): the first blocks transform one each, the
+// others take `rows` rows of a token's A, x comes straight from memory.
+// Columns of a matrix: a cluster of eight CTAs a column.  The elements of a column lie a row of X apart, a 32-byte sector
 // each, so every CTA fetches an eighth and they exchange it through distributed shared memory (each fetching all of it,
 // 272 CTAs of a batch of 16 at N = 4096 moved 35 MB through L2 and took 8 us).  Rank 0 transforms, the others divide A.
 template <bool CLUSTER, int LOGK>
@@ -316,11 +317,13 @@ lora_front_kernel(const __nv_bfloat16 *X, const __nv_bfloat16 *A, const int *ind
     pdl_launch_dependents();
     constexpr int K = 1 << LOGK;
     if constexpr (!CLUSTER) {
-        if (blockIdx.x == 0) {
-            fwht_token<LOGK>((float *)smem_row, X, Xt, scale, nullptr);
+        if ((int)blockIdx.x < columns) {
+            const size_t at = (size_t)blockIdx.x << LOGK;
+            fwht_token<LOGK>((float *)smem_row, X + at, Xt + at, scale, nullptr);
         } else {
-            const int a = index[0];
-            shrink_rows<float>(X, 1, 0, A, a, (unsigned)a < (unsigned)adapters, scaling, S, nullptr, K, rank, (blockIdx.x - 1) * rows, rows);
+            const int groups = (rank + rows - 1) / rows, i = blockIdx.x - columns, t = i / groups, a = index[t];
+            shrink_rows<float>(X, 1, (size_t)t << LOGK, A, a, (unsigned)a < (unsigned)adapters, scaling, S + (size_t)t * rank, nullptr, K,
+                               rank, (i - t * groups) * rows, rows);
         }
         return;
     }
@@ -668,17 +671,18 @@ static int launch_shrink_tiles(const void *X, const void *A, const int *index, c
                               split, status_word_ptr());
 }
 
-static int launch_front(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S, int columns,
-                        int N, float scale, int adapters, int rank, cudaStream_t st)
+static int launch_front(const void *X, bool token_major, const void *A, const int *index, const float *scaling, __nv_bfloat16 *Xt, float *S,
+                        int columns, int N, float scale, int adapters, int rank, cudaStream_t st)
 {
     return with_logk<8>(ilog2((uint32_t)N), [&](auto logk) {
         constexpr int LOGK = decltype(logk)::value < 14 ? decltype(logk)::value : 13;   // the streaming GEMV ends at 8192
-        if (columns == 1) {
-            const int rows = shrink_rows_of_block(1, rank), smem = N * 4;
+        if (token_major || columns == 1) {
+            const int rows = shrink_rows_of_block(columns, rank), smem = N * 4;
             int rc = ensure_dyn_smem((const void *)lora_front_kernel<false, LOGK>, smem);
             if (rc) return rc;
-            return launch_pdl(lora_front_kernel<false, LOGK>, dim3((unsigned)(1 + (rank + rows - 1) / rows)), dim3(256), (size_t)smem, st,
-                              (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, 1, scale, adapters, rank, rows);
+            return launch_pdl(lora_front_kernel<false, LOGK>, dim3((unsigned)(columns * (1 + (rank + rows - 1) / rows))), dim3(256),
+                              (size_t)smem, st, (const __nv_bfloat16 *)X, (const __nv_bfloat16 *)A, index, scaling, Xt, S, columns, scale,
+                              adapters, rank, rows);
         }
         int rows = 1;   // rows of A at a time, of the seventh that a CTA has
         while (rows < 8 && rows < (rank + 6) / 7) rows *= 2;
@@ -692,6 +696,18 @@ static int launch_front(const void *X, const void *A, const int *index, const fl
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// A decoding batch of B columns (or, token_major, tokens) of N elements in two launches: H(X) and S, then the streaming GEMV.
+static int lora_stream(const void *W, const void *X, bool token_major, void *Y, size_t y_row, size_t y_column, const void *A, const void *Bm,
+                       const int *index, const float *scaling, int M, int N, int B, int adapters, int rank, int out_dtype, float scale,
+                       void *workspace, cudaStream_t st)
+{
+    __nv_bfloat16 *Xt = (__nv_bfloat16 *)workspace;
+    float *S = (float *)((unsigned char *)workspace + up256((size_t)N * B * 2));
+    const int rc = launch_front(X, token_major, A, index, scaling, Xt, S, B, N, scale, adapters, rank, st);
+    if (rc) return rc;
+    return launch_gemv_adapt(W, Xt, Y, M, N, B, out_dtype, GemvAdapt{Bm, S, index, adapters, rank, y_row, y_column}, st);
+}
 
 static int check_lora(int M, int N, int K, int adapters, int rank, int out_dtype)
 {
@@ -708,8 +724,10 @@ extern "C" size_t b200ht_lora_gemm_workspace_bytes(int M, int N, int K, int rank
 {
     using namespace b200ht;
     if (M <= 0 || N <= 0 || K <= 0 || rank <= 0) return 0;
-    return b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16) + up256((size_t)N * lora_pitch(rank) * 2) +
-           up256(((size_t)N + 255) / 256 * kLoraTileInts * sizeof(int));
+    // H(X); S in bf16 and the tables, or (few tokens) S in fp32
+    const size_t s16 = up256((size_t)N * lora_pitch(rank) * 2) + up256(((size_t)N + 255) / 256 * kLoraTileInts * sizeof(int));
+    const size_t s32 = gemv_adapt_shape(K, N) ? up256((size_t)N * rank * sizeof(float)) : 0;
+    return b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16) + (s16 > s32 ? s16 : s32);
 }
 
 extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const void *A, const void *B, const int *index,
@@ -729,11 +747,13 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     if ((uintptr_t)workspace & 255u) return B200HT_ERR_ALIGN;
     rc = check_device();
     if (rc) return rc;
-    // one token: the layouts of both entries are the same, and the streaming GEMV is the faster form
-    if (N == 1 && !signs && gemv_adapt_shape(K, 1))
-        return b200ht_lora_gemv(W, X, C, A, B, index, scaling, M, K, 1, adapters, rank, out_dtype, scale, workspace, workspace_bytes,
-                                stream);
     cudaStream_t st = (cudaStream_t)stream;
+    // as few tokens as the streaming GEMV serves with one pass over W: 17 us for 16 of them at 4096 x 4096, 24 by what follows
+    if (!signs && gemv_adapt_shape(K, N)) {
+        const bool mn = out_layout == B200HT_OUT_MN;
+        return lora_stream(W, X, true, C, mn ? (size_t)N : 1, mn ? 1 : (size_t)M, A, B, index, scaling, M, K, N, adapters, rank, out_dtype,
+                           scale, workspace, st);
+    }
     unsigned char *ws = (unsigned char *)workspace + b200ht_fused_gemm_workspace_bytes(M, N, K, B200HT_BF16);
     __nv_bfloat16 *S = (__nv_bfloat16 *)ws;
     int *tiles = (int *)(ws + up256((size_t)N * lora_pitch(rank) * 2));
@@ -773,13 +793,8 @@ extern "C" int b200ht_lora_gemv(const void *W, const void *X, void *Y, const voi
     rc = check_device();
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    if (gemv_adapt_shape(N, B)) {
-        __nv_bfloat16 *Xt = (__nv_bfloat16 *)workspace;
-        float *S = (float *)((unsigned char *)workspace + up256((size_t)N * B * 2));
-        rc = launch_front(X, A, index, scaling, Xt, S, B, N, scale, adapters, rank, st);
-        if (rc) return rc;
-        return launch_gemv_adapt(W, Xt, Y, M, N, B, out_dtype, GemvAdapt{Bm, S, index, adapters, rank}, st);
-    }
+    if (gemv_adapt_shape(N, B))
+        return lora_stream(W, X, false, Y, (size_t)B, 1, A, Bm, index, scaling, M, N, B, adapters, rank, out_dtype, scale, workspace, st);
     float *base = (float *)workspace, *S = (float *)((unsigned char *)workspace + up256((size_t)M * B * sizeof(float)));
     rc = launch_shrink_rows(X, A, index, scaling, S, B, N, adapters, rank, B, false, st);
     if (rc) return rc;

@@ -39,6 +39,7 @@ struct GemvAdapt {
     const float *S;      // [columns][rank]
     const int *index;    // adapter of each column
     int adapters, rank;
+    size_t y_row, y_column;   // strides of the result in elements: one row of W, one column of X
 };
 
 }  // namespace b200ht

@@ -62,7 +62,9 @@ def _check_common(q, positions, inv_freq, sections, axis_order, hadamard):
         raise RuntimeError("rotary: queries and keys must be CUDA tensors")
     if q.dim() != 3:
         raise RuntimeError("rotary: expected queries of shape (tokens, heads, head_dim)")
-    tokens, _, D = q.shape
+    tokens, heads, D = q.shape
+    if tokens >= 1 << 31 or heads >= 1 << 31:
+        raise RuntimeError("rotary: at most 2^31 - 1 tokens and heads")
     if D < 2 or D > 256 or D % 2:
         raise RuntimeError(f"rotary: head_dim must be even and at most 256, got {D}")
     if hadamard and not _is_pow2(D):

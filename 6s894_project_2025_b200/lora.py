@@ -35,6 +35,8 @@ def _check(what: str, X, W, A, B, index, scaling, tokens: int, K: int, out_dtype
     if adapters < 1 or rank < 8 or rank > 128 or rank % 8:
         raise RuntimeError(f"{what}: the rank must be a multiple of 8 up to 128 (pad with zeros) of at least one adapter, got "
                            f"{adapters} of rank {rank}")
+    if max(tokens, M, adapters) >= 1 << 31:
+        raise RuntimeError(f"{what}: at most 2^31 - 1 tokens, rows and adapters")
     if index.dtype != torch.int32 or index.dim() != 1 or index.shape[0] != tokens:
         raise RuntimeError(f"{what}: index must be {tokens} int32 entries")
     if scaling is not None:
