@@ -424,14 +424,14 @@ lora_expand_kernel(const float *base, const __nv_bfloat16 *B, const float *S, co
 constexpr int kShrinkStages = 3, kShrinkThreads = 320;
 constexpr int kShrinkXBytes = 256 * 128, kShrinkStageBytes = 2 * kShrinkXBytes;
 constexpr int kShrinkSmem = kShrinkStages * kShrinkStageBytes + 1024 + 128;
-static_assert(256 * (kLoraMaxRank + 1) * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
+static_assert(256 * kLoraMaxRank * 4 <= kShrinkStages * kShrinkStageBytes, "the partial sums lie over the stages");
 
-__device__ __forceinline__ float cluster_load(uint32_t local, int rank)   // the float at `local` in the shared memory of CTA `rank`
+__device__ __forceinline__ float4 cluster_load4(uint32_t local, int rank)   // from `local` in the shared memory of CTA `rank`
 {
-    float v;
+    float4 v;
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
 
@@ -497,8 +497,8 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
     __syncthreads();
     const int count = count_s;
     const int share = 128 / rank;                   // adapters of one instruction
-    float *partial = (float *)gen;                  // [256][rank + 1], over the stages
-    const int pitch = rank + 1, out_pitch = lora_pitch(rank);
+    float *partial = (float *)gen;                  // [256][rank], over the stages
+    const int out_pitch = lora_pitch(rank);
     const int rows = 256 / split, row0 = part * rows;   // tokens whose sums this CTA writes
     if (blockIdx.y == 0)                            // tokens without an adapter
         for (int i = tid; i < rows * (rank / 8); i += kShrinkThreads) {
@@ -573,23 +573,26 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (slot[c + i] == mine) partial[(c + i) * pitch + r] = __uint_as_float(v[i]);
+                        if (slot[c + i] == mine) partial[(c + i) * rank + r] = __uint_as_float(v[i]);
                 }
             }
             tc_fence_before();
         }
         cluster_sync_all();
-        for (int i = tid; i < rows * rank && ok; i += kShrinkThreads) {
-            const int row = row0 + i / rank, r = i % rank, mine = slot[row] - first;
+        const int fours = rank / 4;
+        for (int i = tid; i < rows * fours && ok; i += kShrinkThreads) {
+            const int row = row0 + i / fours, r = i % fours * 4, mine = slot[row] - first;
             if (mine < 0 || mine >= n) continue;
-            const uint32_t at = base + (uint32_t)((row * pitch + r) * 4);
-            float v[8], sum = 0.f;
-#pragma unroll
-            for (int p = 0; p < 8; ++p) v[p] = p < split ? cluster_load(at, p) : 0.f;
+            const uint32_t at = base + (uint32_t)((row * rank + r) * 4);
+            float4 v[8], sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int p = 0; p < 8; ++p)
-                if (p < split) sum += v[p];
-            S[(size_t)(t0 + row) * out_pitch + r] = __float2bfloat16_rn(sum * factor[row]);
+                if (p < split) v[p] = cluster_load4(at, p);
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < split) sum = make_float4(sum.x + v[p].x, sum.y + v[p].y, sum.z + v[p].z, sum.w + v[p].w);
+            const float f = factor[row];
+            *(uint2 *)(S + (size_t)(t0 + row) * out_pitch + r) = make_uint2(pack2<B200HT_BF16>(sum.x * f, sum.y * f), pack2<B200HT_BF16>(sum.z * f, sum.w * f));
         }
         fence_proxy_async();   // the next pass' copies overwrite what was read here
         cluster_sync_all();

@@ -771,13 +771,14 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
     }
 }
 
-// dw[i] = sum of the blocks' rows, in a fixed order: 8 warps take every eighth row of 32 columns, then the warps are
-// added in order.  blockIdx.y: queries or keys.
+// dw[i] = sum of the blocks' rows, in a fixed order: 32 warps take every 32nd row of 32 columns, then the warps are
+// added in order.  blockIdx.y: queries or keys.  (Eight warps took 6 us longer: each row is a trip to L2.)
+constexpr int kSumWarps = 32;
 template <int DT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(32 * kSumWarps)
 norm_weight_grad_kernel(const float *partial, int q_blocks, int k_blocks, int D, void *dwq, void *dwk, int w_f32)
 {
-    __shared__ float part[8][32];
+    __shared__ float part[kSumWarps][32];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -786,13 +787,14 @@ norm_weight_grad_kernel(const float *partial, int q_blocks, int k_blocks, int D,
     const int n = blockIdx.y ? k_blocks : q_blocks;
     float s = 0.f;
     if (i < D)
-        for (int r = warp; r < n; r += 8) s += rows[(long long)r * D + i];
+#pragma unroll 8
+        for (int r = warp; r < n; r += kSumWarps) s += rows[(long long)r * D + i];
     part[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && i < D) {
         s = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) s += part[w][lane];
+        for (int w = 0; w < kSumWarps; ++w) s += part[w][lane];
         void *dw = blockIdx.y ? dwk : dwq;
         if (w_f32) ((float *)dw)[i] = s;
         else rot_store<DT>(dw, i, s);
@@ -988,7 +990,7 @@ static int launch_norm_grad(RotArgs &a, bool had, void *dwq, void *dwk, cudaStre
         rc = launch_row_grad<DT, 16>(a, had, mode, &b, st);
     }
     if (rc) return rc;
-    return launch_pdl(norm_weight_grad_kernel<DT>, dim3((unsigned)((a.D + 31) / 32), 2), dim3(256), 0, st, (const float *)a.partial,
+    return launch_pdl(norm_weight_grad_kernel<DT>, dim3((unsigned)((a.D + 31) / 32), 2), dim3(32 * kSumWarps), 0, st, (const float *)a.partial,
                       b.q, b.k, a.D, dwq, dwk, a.w_f32);
 }
 
