@@ -441,7 +441,7 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
 {
     extern __shared__ unsigned char smem_dyn[];
     __shared__ TileAdapters found;
-    __shared__ int list[256], slot[256];   // the tile's adapters; each token's place among them
+    __shared__ __align__(16) int list[256], slot[256];   // the tile's adapters; each token's place among them
     __shared__ float factor[256];          // scaling of each token's adapter
     __shared__ int count_s;
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
@@ -488,9 +488,10 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
         int id = t0 + t < tokens ? __ldcg(index + t0 + t) : -1, mine;
         if ((unsigned)id >= (unsigned)adapters) id = -1;
         bool first;
-        factor[t] = scaling && id >= 0 ? scaling[id] : 1.f;
+        const float f = scaling && id >= 0 ? scaling[id] : 1.f;   // under way while the adapters are found
         const int n = tile_adapters(found, t, id, mine, first, [] { asm volatile("bar.sync 1, 256;\n" ::: "memory"); });
         slot[t] = mine;
+        factor[t] = f;
         if (first) list[mine] = id;
         if (t == 0) count_s = n;
     }
@@ -568,12 +569,20 @@ lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_co
                 const int mine = a < share && g * share + a < n ? first + g * share + a : -2;   // -2 is no token's place
 #pragma unroll 1
                 for (int c = c0; c < c0 + 128; c += 32) {
-                    uint32_t v[32];
+                    uint32_t v[32], keep = 0;   // bit i: token c + i is this adapter's
                     tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + g * 256 + c, v);
+                    // all places before the first store, which would hold back the loads behind it
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int4 p = *(const int4 *)(slot + c + 4 * i);
+                        keep |= (p.x == mine ? 1u : 0u) << (4 * i) | (p.y == mine ? 2u : 0u) << (4 * i) | (p.z == mine ? 4u : 0u) << (4 * i) |
+                                (p.w == mine ? 8u : 0u) << (4 * i);
+                    }
                     tmem_ld_wait();
+                    float *to = partial + c * rank + r;
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (slot[c + i] == mine) partial[(c + i) * rank + r] = __uint_as_float(v[i]);
+                        if ((keep >> i) & 1u) to[i * rank] = __uint_as_float(v[i]);
                 }
             }
             tc_fence_before();

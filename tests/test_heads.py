@@ -196,6 +196,8 @@ SHAPES = [
     (1, 1, 1, 2, 1), (1, 32, 8, 128, 64), (3, 5, 1, 64, 32), (17, 28, 4, 128, 64), (2, 3, 3, 80, 40), (7, 4, 2, 96, 48),
     (5, 2, 1, 256, 32), (4, 16, 2, 256, 128), (9, 3, 2, 128, 32), (3, 2, 2, 36, 18), (6, 7, 1, 66, 20), (33, 1, 0, 64, 32),
     (130, 9, 3, 128, 60), (5, 2, 2, 112, 24), (70, 6, 6, 32, 16), (19, 5, 5, 16, 8),
+    # enough tokens that a block takes several of them, with heads that leave some of its groups idle
+    (301, 28, 4, 128, 64), (333, 5, 3, 64, 32), (310, 3, 1, 256, 128), (401, 16, 16, 80, 40), (299, 1, 7, 96, 24),
 ]
 
 
@@ -457,3 +459,58 @@ def test_results_lie_between_untouched_zones(pkg, lib):
         for o, view in zip(outs, (qo, ko)):
             view.fill_(7.0)
             assert bool((o == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(pkg):
+    """Rows 32768 elements apart: the last tokens lie behind element 2^31."""
+    T, row = 65600, 32768
+    big = torch.empty(T * row, dtype=torch.bfloat16, device="cuda")
+    q, k = big.as_strided((T, 2, 128), (row, 128, 1)), big.as_strided((T, 1, 128), (row, 128, 1), 512)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q.copy_(torch.randn(T, 2, 128, generator=g, device="cuda"))
+    k.copy_(torch.randn(T, 1, 128, generator=g, device="cuda"))
+    pos, inv = torch.arange(T, device="cuda"), (1e4 ** (-torch.arange(64, dtype=torch.float64) / 64)).float().cuda()
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    last = slice(T - 70, T)
+    want = [forward64(x[last], w, 1e-6, pos[last], inv, hadamard=True) for x in (q, k)]
+    grads = pkg.norm_rotary_qk_backward(q, k, q, k, w, w, pos, inv)
+    got = pkg.norm_rotary_qk(q, k, w, w, pos, inv, hadamard=True, inplace=True)
+    for a, b in zip(got, want):
+        assert_close(a[last], b)
+    assert torch.isfinite(grads[0]).all() and grads[0].shape == q.shape
+    # a kernel for other alignments walks the same offsets
+    odd = big.as_strided((T, 1, 66), (row, 66, 1), 1001)
+    odd.copy_(torch.randn(T, 1, 66, generator=g, device="cuda"))
+    want = forward64(odd[last], None, 0, pos[last], inv[:33])
+    assert_close(pkg.rotary_qk(odd, None, pos, inv[:33])[0][last], want)
+
+
+@pytest.mark.gpu
+def test_gradients_captured_in_a_graph(pkg):
+    """A training step captured by torch.autograd.grad: forward, backward and replay with other values in the leaves."""
+    q, k, pos, inv = make(40, 4, 2, 64, 32, torch.bfloat16, far=60)
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, w, w)]
+
+    def step():
+        out = torch.ops.b200ht.norm_rotary_qk(*leaves, pos, inv, 1e-6, None, "blocks", False, True)
+        return torch.autograd.grad(out, leaves, (dq, dk))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        leaves[0].copy_(q.flip(0))
+    with torch.cuda.stream(s):
+        graph.replay()
+    torch.cuda.synchronize()
+    want = pkg.norm_rotary_qk_backward(dq, dk, q.flip(0), k, w, w, pos, inv, hadamard=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -435,3 +435,29 @@ def test_another_stream_than_the_current_one_waits_its_turn(pkg):
                 t.zero_()
             assert all(torch.equal(u, v) for u, v in zip(got, want))
     assert pkg.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_results_beyond_32_bits(pkg):
+    """More than 2^31 elements of C, the tokens in many chunks' worth of tiles: looked at near its end."""
+    N, K, M = 66000, 64, 32768
+    g = torch.Generator(device="cuda").manual_seed(17)
+    X, W = (torch.randn(n, K, generator=g, device="cuda").bfloat16() for n in (N, M))
+    A, B = torch.randn(5, 8, K, generator=g, device="cuda").bfloat16(), torch.randn(5, M, 8, generator=g, device="cuda").bfloat16()
+    index = (torch.arange(N, device="cuda") // 300 % 6 - 1).int()
+    got = pkg.lora_ht_gemm(X, W, A, B, index, out_layout="nm", out_dtype=torch.bfloat16)
+    last = slice(N - 600, N)
+    small = pkg.lora_ht_gemm(X[last], W, A, B, index[last], out_layout="nm", out_dtype=torch.float32)
+    assert pkg.device_status() == 0
+    # The same sums in another order at most: K / 16 + 2 additions of 2^-22 each of the sizes' sum, and the rounding to bf16.
+    # S comes from another kernel for so few tokens: both sums are within (K + 1) 2^-24 of the sizes of the true one, and
+    # each is rounded to bf16, 2^-8 of its value, so that the two S differ by twice that at most (in the sizes of B S).
+    _, s_unit, share = share64(X[last], A, B, index[last], None)
+    h = torch.ones(1, 1, dtype=torch.float64)
+    while h.shape[0] < K:
+        h = torch.cat([torch.cat([h, h], 1), torch.cat([h, -h], 1)])
+    size = share + ((X[last].double().cpu() @ h).abs() / 8) @ W.double().cpu().abs().t()
+    room = size * (K / 16 + 2) * 2.0 ** -22 + 2 * (share * 2.0 ** -8 + (K + 1) * U * s_unit)
+    want = small.double().cpu()
+    off = (got[last].double().cpu() - want).abs()
+    assert bool((off <= room + (want.abs() + room) * 2.0 ** -8).all())
