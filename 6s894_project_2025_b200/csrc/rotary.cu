@@ -578,15 +578,15 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t from)   // volatile: not
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
     return v;
 }
-// Vector s of a row in its slot, as fp32.
+// Vector s of a row in its slot, as fp32.  `from`: 16 bits, the lane's first vector, the second 16 bytes a thread on; fp32,
+// where the group's row begins, in its natural order, with `at` = byte of the lane's vector s.
 template <int DT>
-__device__ __forceinline__ void slot_vector(uint32_t from, int s, float2 (&v)[4])
+__device__ __forceinline__ void slot_vector(uint32_t from, int s, int at, float2 (&v)[4])
 {
-    constexpr int VECS = DT == B200HT_F32 ? 2 : 1;
     if constexpr (DT == B200HT_F32) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint4 r = load_shared16(from + (s * VECS + i) * kRowThreads * 16);
+            const uint4 r = load_shared16(from + at + 16 * i);
             v[2 * i] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
             v[2 * i + 1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
         }
@@ -620,7 +620,11 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
     const int steps = (t.heads + per - 1) / per;
     const int partner = row_partner(MODE, j, a.pairs);
     const float hc = HAD ? rsqrtf((float)D) : 1.f, inv_d = 1.f / (float)D;
-    const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+    // 16 bits: a lane copies the two vectors that it will read.  fp32: the lanes copy 16 bytes side by side, whole sectors
+    // (their own 32 bytes would be two requests for half a sector each, and every sector would cross to the SM twice)
+    const uint32_t slots = (uint32_t)__cvta_generic_to_shared(smem);
+    const uint32_t copy_to = slots + (VECS == 2 ? group * LANES * 64 + j * 16 : threadIdx.x * 16);
+    const uint32_t read_at = slots + (VECS == 2 ? group * LANES * 64 : threadIdx.x * 16);
     float2 *tab = (float2 *)(smem + kRowSlots * SLOT) + warp * tokens * half;
     pdl_launch_dependents();
     pdl_wait();
@@ -642,20 +646,27 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
     int f_step = 0, f_left, slot = 0;
     auto row = [&]() {
         const long long token = f_first + tk;
-        f_left = token < a.tokens && j < lanes ? t.heads - h0 : 0;
-        fx = (const unsigned char *)t.x + (token * t.x_tok + h0 * t.x_head + 8 * j) * SIZE;
-        fg = (const unsigned char *)t.g + (token * t.g_tok + h0 * t.g_head + 8 * j) * SIZE;
+        f_left = token < a.tokens && (VECS == 2 || j < lanes) ? t.heads - h0 : 0;
+        fx = (const unsigned char *)t.x + (token * t.x_tok + h0 * t.x_head) * SIZE + 16 * j;
+        fg = (const unsigned char *)t.g + (token * t.g_tok + h0 * t.g_head) * SIZE + 16 * j;
     };
     auto fetch = [&](int to_slot) {
         if (f_left > 0) {
-            const uint32_t to = mine_s + to_slot * SLOT;
+            const uint32_t to = copy_to + to_slot * SLOT;
+            if constexpr (VECS == 2) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+                for (int c = 0; c < 4; ++c)
+                    if (c * LANES + j < 4 * lanes) {
+                        copy_async16(to + c * LANES * 16, fx + c * LANES * 16);
+                        copy_async16(to + SLOT / 2 + c * LANES * 16, fg + c * LANES * 16);
+                    }
+            } else {
 #pragma unroll
-                for (int i = 0; i < VECS; ++i) {
-                    copy_async16(to + (s * VECS + i) * kRowThreads * 16, fx + s * half * SIZE + 16 * i);
-                    copy_async16(to + ((2 + s) * VECS + i) * kRowThreads * 16, fg + s * half * SIZE + 16 * i);
+                for (int s = 0; s < 2; ++s) {
+                    copy_async16(to + s * kRowThreads * 16, fx + s * half * SIZE);
+                    copy_async16(to + SLOT / 2 + s * kRowThreads * 16, fg + s * half * SIZE);
                 }
+            }
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
         if (++f_step == steps) {
@@ -683,14 +694,16 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
         unsigned char *y = (unsigned char *)t.y + (token * t.y_tok + h0 * t.y_head + 8 * j) * SIZE;
 #pragma unroll 1
         for (int step = 0; step < steps; ++step) {
+            if (VECS == 2) __syncwarp();   // all lanes have read the slot that is filled now
             fetch(slot == 0 ? kRowSlots - 1 : slot - 1);
             asm volatile("cp.async.wait_group %0;\n" ::"n"(kRowSlots - 1) : "memory");
+            if (VECS == 2) __syncwarp();   // and all have their copies here
             const bool on = left > 0;
-            const uint32_t from_x = mine_s + slot * SLOT, from_g = from_x + 2 * VECS * kRowThreads * 16;
+            const uint32_t from_x = read_at + slot * SLOT, from_g = from_x + SLOT / 2;
             slot = slot + 1 == kRowSlots ? 0 : slot + 1;
             float2 g[2][4];
-            slot_vector<DT>(from_g, 0, g[0]);
-            slot_vector<DT>(from_g, 1, g[1]);
+            slot_vector<DT>(from_g, 0, 32 * jj, g[0]);
+            slot_vector<DT>(from_g, 1, half * 4 + 32 * jj, g[1]);
             if (HAD) row_hadamard<LANES>(g, j, lanes);
             if constexpr (MODE == kPairsHalves) {
 #pragma unroll
@@ -712,7 +725,7 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 float2 x[4];
-                slot_vector<DT>(from_x, s, x);
+                slot_vector<DT>(from_x, s, s * half * 4 + 32 * jj, x);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) q = fma2(x[i], x[i], q);
             }
@@ -722,7 +735,7 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 float2 x[4];
-                slot_vector<DT>(from_x, s, x);
+                slot_vector<DT>(from_x, s, s * half * 4 + 32 * jj, x);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float4 f = row_weights(wts, s, i, jj, lanes);
@@ -743,7 +756,7 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     float2 x[4];
-                    slot_vector<DT>(from_x, s, x);
+                    slot_vector<DT>(from_x, s, s * half * 4 + 32 * jj, x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         g[s][i] = fma2(x[i], make_float2(k, k), mul2(g[s][i], make_float2(rc, rc)));
