@@ -18,8 +18,6 @@
 
 namespace b200ht {
 
-int launch_fwht(const void *in, void *out, uint64_t rows, uint32_t n, int dtype, float scale, const void *signs,
-                cudaStream_t st, int keep_out);
 int launch_gemv_adapt(const void *W, const void *Xt, void *Y, int M, int N, int B, int out_dtype, const GemvAdapt &adapt,
                       cudaStream_t st);
 bool gemv_adapt_shape(int N, int B);
@@ -106,7 +104,8 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const int *index, int to
 //   A  32 consecutive values a thread from global memory: bits 0 .. 4 of the index
 //   B  rounds of up to five bits from bit 5 on, lanes side by side (one for K = 8192, two beyond)
 //   C  8 consecutive values and the last three bits: scaled, rounded, stored as 16-byte vectors
-// Bound: HBM, then shared memory (16 bytes an element and round).
+// Bound: shared memory and the instruction rate (0.63 issued a cycle): 2048 tokens of 8192 in 19 us (10 at the copy
+// bandwidth, fwht.cu 12); with the places computed element by element 32 us.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int line_at(int e)   // place of element e
 {
@@ -412,7 +411,8 @@ lora_expand_kernel(const float *base, const __nv_bfloat16 *B, const float *S, co
 // Each token keeps the rows of its own adapter.  With prompts a tile has a few adapters, one pass serves them and X is read
 // once; bound then: the bytes of X.  (An instruction takes about 90 ns whatever its M and N, so it should be full: with 128
 // tokens as M and an instruction an adapter, 16384 x 8192 tokens of 40 requests at rank 64 took 94 us; with the adapters as
-// M and 128 tokens as N, 97 us, two tiles an SM taking turns and a second pass where a tile had three adapters.)
+// M and 128 tokens as N, 97 us, two tiles an SM taking turns and a second pass where a tile had three adapters; so 71 us,
+// 41 at the copy bandwidth.)  Short prompts are bound by the chain of latencies: 2001 x 4096 at rank 32 takes 14 us.
 //
 // Warp 0 copies by TMA (X 256 x 64 and rank x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the MMAs,
 // warps 2..9 find the tile's adapters while the first tiles of X arrive, and at the end bring the accumulators (one row of
@@ -655,9 +655,9 @@ int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale
     });
 }
 
-// Few tokens: a block for each, which reads its A through L2 (5 TB/s or so, whatever the tokens' order); from 32 MB of such
-// reads on the tile kernel, which needs about 12 us for a few adapters a tile and 15 more for each further pass.  At 256
-// tokens, K = 4096, rank 16 (32 MB): 7 us against 13 (one adapter) and 29 (64 adapters).
+// Few tokens: blocks for each, which read its A through L2 (3 TB/s or so, whatever the tokens' order); from 32 MB of such
+// reads on the tile kernel, whose time goes by the adapters of a tile.  At 256 tokens, K = 4096, rank 16 (32 MB): 12 us
+// against 13 (one adapter) and 29 (64 adapters).
 static bool shrink_by_rows(int tokens, int K, int rank) { return (size_t)tokens * rank * K * 2 <= (size_t)32 << 20; }
 
 static int launch_shrink_tiles(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int K,

@@ -85,7 +85,8 @@ __device__ __forceinline__ float warp_sum(float v)
 
 // ---------------------------------------------------------------------------
 // Any head dimension, stride and alignment: a warp per row, the row in shared memory as fp32, one element per lane and
-// step.
+// step.  About ten times slower than the fast form below (32768 x 40 x 128 with H: 1460 us against 138), for rows that it
+// does not take.
 // ---------------------------------------------------------------------------
 constexpr int kAnyWarps = 4;
 
@@ -218,8 +219,10 @@ norm_rotary_any_grad_kernel(const __grid_constant__ RotArgs a, int q_blocks)
 // 8j .. 8j + 7 and head_dim / 2 + the same, so both members of a split pair, and the top bit of the index for H, meet in
 // one lane; H needs shuffles for log2(head_dim) - 4 bits only.  A block of 256 threads takes `tb` tokens: cos and sin of
 // their pairs are computed once into shared memory and serve all heads, each group walks over heads of one token with
-// the next row's loads in flight.  Bound: HBM; with H the instruction rate is next (about 200 issued instructions per
-// 512 values and warp), hence the packed fp32 instructions.
+// the next row's loads in flight.  Bound: HBM without H, the instruction rate with it (160 issued instructions per 512
+// values and warp, 330 with H), hence the packed fp32 instructions: 66 us against 73 without them.
+// 16384 tokens x 40 heads x 128, bf16 (51 us at the copy bandwidth): rotation 62 us, with H 66, norm 65, norm with H 76; four
+// resident blocks an SM (64 registers) measured best, three 65 / 70 / 68 / 77, five spill (68 / 104 / 92 / 122).
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
@@ -566,8 +569,9 @@ rotary_row_kernel(const __grid_constant__ RotArgs a, int tb, int mode)
 // keys.  A warp takes whole tokens (per = 32 / LANES / tokens-of-a-warp groups each) and needs no other warp until the
 // end, where the block's share of the weights' gradient, in registers so far, is added up: with barriers around the
 // table of cos and sin the blocks stood still for a fifth of the time.  Registers are what limits it: the next row comes
-// by cp.async into a slot of shared memory that its own thread alone reads, x is read from there once for each of its
-// three uses, and for split pairs cos and sin stay in shared memory as well.
+// by cp.async into a slot of shared memory that its own thread (fp32: group) alone reads, x is read from there once for
+// each of its three uses, and for split pairs cos and sin stay in shared memory as well.  16384 tokens x 40 heads x 128,
+// bf16: 90 us, 77 at the copy bandwidth; 127 with H (instruction rate).
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void *src)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
