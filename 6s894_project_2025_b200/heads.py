@@ -124,7 +124,7 @@ def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
     if gap >= reach(q) * size or -gap >= reach(k) * size:
         return True
     row = q.stride(0)
-    if row != k.stride(0) or gap % size:
+    if row != k.stride(0) or gap % size or row == 0:   # 0: one token, seen through expand
         return False
     # within one row of the packed tensor: q's heads at 0, the keys' at `at`
     at = gap // size % row

@@ -155,6 +155,15 @@ def test_shared_memory_is_found(pkg):
     assert not heads._apart(x[:4], x[3:]) and not heads._apart(x[:, :4], x.transpose(0, 1)[:6])
 
 
+def test_shared_memory_of_one_expanded_token_is_found(pkg):
+    """A token's stride may be zero where there is only one."""
+    import importlib
+    heads = importlib.import_module("6s894_project_2025_b200.heads")
+    x = torch.zeros(8, 16).as_strided((1, 8, 16), (0, 16, 1))
+    assert heads._apart(x[:, :4], x[:, 4:]) and heads._apart(x[:, 4:], x[:, :4])
+    assert not heads._apart(x[:, :4], x[:, 3:]) and not heads._apart(x[:, 3:], x[:, :4])
+
+
 def test_c_entries_refuse_before_the_gpu(lib):
     l = lib.load()
     buf = ctypes.create_string_buffer(4096)
