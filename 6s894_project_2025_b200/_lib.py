@@ -121,6 +121,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
     header.  The build takes a file lock: ranks started together do not compile the same objects twice.
     """
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -92,11 +92,12 @@ def _check_common(q, positions, inv_freq, sections, axis_order, hadamard):
 
 
 def _check_weights(q, q_weight, k_weight, D):
-    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w.dim() != 1 or w.shape[0] != D or w.device != q.device:
-            raise RuntimeError(f"norm_rotary_qk: {what} must be a vector of {D} entries on the queries' device")
-        if w.dtype not in (q.dtype, torch.float32) or w.dtype != q_weight.dtype:
-            raise RuntimeError("norm_rotary_qk: the weights must both have the queries' dtype, or both be float32")
+    device, dtype = q.device, q_weight.dtype
+    for w in (q_weight, k_weight):
+        if tuple(w.shape) != (D,) or w.device != device:
+            raise RuntimeError(f"norm_rotary_qk: the weights must be vectors of {D} entries on the queries' device")
+    if k_weight.dtype != dtype or dtype != q.dtype and dtype != torch.float32:
+        raise RuntimeError("norm_rotary_qk: the weights must both have the queries' dtype, or both be float32")
 
 
 def _own_memory(x: torch.Tensor) -> bool:
@@ -134,7 +135,8 @@ def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
 def _run(q, k, q_weight, k_weight, eps, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse, inplace):
     D, tokens, pairs, flags, table, n_axes, pa, pt = _check_common(q, positions, inv_freq, sections, axis_order, hadamard)
     q_in, k_in = q, k
-    q = _check_heads(q, q, "queries")
+    if q.stride(2) != 1:
+        q = q.contiguous()
     if k is not None:
         k = _check_heads(k, q, "keys")
     if q_weight is not None:
@@ -214,7 +216,9 @@ def norm_rotary_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
     in an order that depends on the sizes alone.
     """
     D, tokens, pairs, flags, table, n_axes, pa, pt = _check_common(q, positions, inv_freq, sections, axis_order, hadamard)
-    q, k = _check_heads(q, q, "queries"), _check_heads(k, q, "keys")
+    k = _check_heads(k, q, "keys")
+    if q.stride(2) != 1:
+        q = q.contiguous()
     _check_weights(q, q_weight, k_weight, D)
     if dq_out.shape != q.shape or dk_out.shape != k.shape:
         raise RuntimeError("norm_rotary_qk_backward: the gradients must have the shapes of q and k")
@@ -231,12 +235,13 @@ def norm_rotary_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
     strides = _strides12(*dq_out.stride()[:2], *dk_out.stride()[:2], *q.stride()[:2], *k.stride()[:2], *dq.stride()[:2],
                          *dk.stride()[:2])
     lib = _lib.load()
-    ws = torch.empty(lib.b200ht_norm_rotary_qk_backward_workspace_bytes(D), dtype=torch.uint8, device=q.device)
+    size = lib.b200ht_norm_rotary_qk_backward_workspace_bytes(D)
+    ws = q.new_empty(size // q.element_size())   # cheaper than a tensor of bytes
     with _on_device(q.device):
         rc = lib.b200ht_norm_rotary_qk_backward(
             dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
             float(eps), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), tokens, q.shape[1], k.shape[1], D,
             strides, _DT[q.dtype], positions.data_ptr(), pa, pt, n_axes, table, inv_freq.data_ptr(), pairs, flags,
-            ws.data_ptr(), ws.numel(), _stream_ptr(q.device))
+            ws.data_ptr(), size, _stream_ptr(q.device))
     _lib.check(rc, "b200ht_norm_rotary_qk_backward")
     return dq, dk, dqw, dkw

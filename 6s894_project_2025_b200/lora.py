@@ -54,10 +54,10 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _out(what, out, shape, dtype, device):
+def _out(what, out, shape, dtype, like):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.device != device or out.data_ptr() % 16:
+        return like.new_empty(shape, dtype=dtype)
+    if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.device != like.device or out.data_ptr() % 16:
         raise RuntimeError(f"{what}: out has the wrong shape, dtype, strides, device or alignment")
     return out
 
@@ -85,18 +85,19 @@ def lora_ht_gemm(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Ten
     out_dtype = out_dtype or torch.float32
     M, adapters, rank, A, B, index, scaling = _check("lora_ht_gemm", X, W, A, B, index, scaling, N, K, out_dtype)
     X, W = _rows(X), _rows(W)
-    out = _out("lora_ht_gemm", out, (M, N) if out_layout == "mn" else (N, M), out_dtype, X.device)
+    out = _out("lora_ht_gemm", out, (M, N) if out_layout == "mn" else (N, M), out_dtype, X)
     if M == 0 or N == 0:
         return out
     lib = _lib.load()
     mask = None if signs is None else sign_mask(signs, K, X.device)
-    ws = torch.empty(lib.b200ht_lora_gemm_workspace_bytes(M, N, K, rank), dtype=torch.uint8, device=X.device)
+    size = lib.b200ht_lora_gemm_workspace_bytes(M, N, K, rank)
+    ws = X.new_empty(size // 2)   # cheaper than a tensor of bytes
     with _on_device(X.device):
         rc = lib.b200ht_lora_gemm(X.data_ptr(), W.data_ptr(), out.data_ptr(), A.data_ptr(), B.data_ptr(), index.data_ptr(),
                                   None if scaling is None else scaling.data_ptr(), M, N, K, adapters, rank, _DT[out_dtype],
                                   _lib.OUT_MN if out_layout == "mn" else _lib.OUT_NM,
                                   math.sqrt(1.0 / K) if scale is None else float(scale),
-                                  None if mask is None else mask.data_ptr(), ws.data_ptr(), ws.numel(), _stream_ptr(X.device))
+                                  None if mask is None else mask.data_ptr(), ws.data_ptr(), size, _stream_ptr(X.device))
     _lib.check(rc, "b200ht_lora_gemm")
     return out
 
@@ -125,14 +126,15 @@ def lora_ht_gemv(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Ten
         return lora_ht_gemm(X.t(), W, A, B, index, scaling=scaling, scale=scale, out_dtype=out_dtype, out=out)
     M, adapters, rank, A, B, index, scaling = _check("lora_ht_gemv", X, W, A, B, index, scaling, columns, N, out_dtype)
     X, W = _rows(X), _rows(W)
-    out = _out("lora_ht_gemv", out, (M, columns), out_dtype, X.device)
+    out = _out("lora_ht_gemv", out, (M, columns), out_dtype, X)
     if M == 0:
         return out
-    ws = torch.empty(lib.b200ht_lora_gemv_workspace_bytes(M, N, columns, rank), dtype=torch.uint8, device=X.device)
+    size = lib.b200ht_lora_gemv_workspace_bytes(M, N, columns, rank)
+    ws = X.new_empty(size // 2)   # cheaper than a tensor of bytes
     with _on_device(X.device):
         rc = lib.b200ht_lora_gemv(W.data_ptr(), X.data_ptr(), out.data_ptr(), A.data_ptr(), B.data_ptr(), index.data_ptr(),
                                   None if scaling is None else scaling.data_ptr(), M, N, columns, adapters, rank,
                                   _DT[out_dtype], math.sqrt(1.0 / N) if scale is None else float(scale), ws.data_ptr(),
-                                  ws.numel(), _stream_ptr(X.device))
+                                  size, _stream_ptr(X.device))
     _lib.check(rc, "b200ht_lora_gemv")
     return out
