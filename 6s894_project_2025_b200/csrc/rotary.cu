@@ -859,6 +859,9 @@ static int check_rot_common(const RotArgs &a, int dtype, int flags, const unsign
     if (flags & ~(B200HT_ROT_INTERLEAVED | B200HT_ROT_HADAMARD | B200HT_ROT_INVERSE | B200HT_ROT_POS64 | B200HT_ROT_WEIGHT_F32))
         return B200HT_ERR_SIZE;
     if (a.tokens < 0 || a.t[0].heads < 0 || a.t[1].heads < 0) return B200HT_ERR_SIZE;
+    // the kernels and their grids count tokens, and both tensors' heads together, in 32 bits, rounded up to a block's share
+    constexpr int kMostRows = (1 << 30) - 1;
+    if (a.tokens > kMostRows || a.t[0].heads > kMostRows || a.t[1].heads > kMostRows) return B200HT_ERR_SIZE;
     if (a.D < 2 || a.D > kMaxHeadDim || (a.D & 1) || a.pairs < 1 || 2 * a.pairs > a.D) return B200HT_ERR_SIZE;
     if ((flags & B200HT_ROT_HADAMARD) && !is_pow2((uint64_t)a.D)) return B200HT_ERR_SIZE;
     if (n_axes < 1 || n_axes > kMaxAxes || (n_axes > 1 && !axis_of_pair)) return B200HT_ERR_SIZE;

@@ -48,6 +48,8 @@ def _check_heads(x: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor
     sx, sl = x.shape, like.shape
     if len(sx) != 3 or sx[0] != sl[0] or sx[2] != sl[2]:
         raise RuntimeError(f"rotary: expected {what} of shape (tokens, heads, head_dim) like the queries")
+    if sx[1] >= 1 << 30:
+        raise RuntimeError("rotary: fewer than 2^30 tokens and heads")
     if x.dtype != like.dtype or x.device != like.device:
         raise RuntimeError(f"rotary: {what} must have the queries' dtype and device")
     return x if x.stride(2) == 1 else x.contiguous()
@@ -63,8 +65,8 @@ def _check_common(q, positions, inv_freq, sections, axis_order, hadamard):
     if q.dim() != 3:
         raise RuntimeError("rotary: expected queries of shape (tokens, heads, head_dim)")
     tokens, heads, D = q.shape
-    if tokens >= 1 << 31 or heads >= 1 << 31:
-        raise RuntimeError("rotary: at most 2^31 - 1 tokens and heads")
+    if tokens >= 1 << 30 or heads >= 1 << 30:
+        raise RuntimeError("rotary: fewer than 2^30 tokens and heads")
     if D < 2 or D > 256 or D % 2:
         raise RuntimeError(f"rotary: head_dim must be even and at most 256, got {D}")
     if hadamard and not _is_pow2(D):

@@ -245,7 +245,8 @@ int b200ht_ipc_close(void *base);
  *                 B200HT_ROT_HADAMARD: . H / sqrt(head_dim) after the rotation (head_dim a power of two)
  *                 B200HT_ROT_INVERSE: the transposed steps in reverse order, which is the gradient (no norm)
  *                 B200HT_ROT_WEIGHT_F32: the weights are floats, not `dtype`
- * head_dim is even, 2 .. 256; dtype F16 | BF16 | F32.  fp32 arithmetic (fp64 for the angle), one rounding on the store.
+ * head_dim is even, 2 .. 256; fewer than 2^30 tokens, query heads and key heads; dtype F16 | BF16 | F32.  fp32 arithmetic
+ * (fp64 for the angle), one rounding on the store.
  * Pointers need the alignment of their element type; 16-byte aligned rows of a multiple of 16 elements run fastest.
  */
 #define B200HT_ROT_INTERLEAVED 1

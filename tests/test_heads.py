@@ -199,6 +199,20 @@ def test_c_entries_refuse_before_the_gpu(lib):
     assert grad(ws=None) == -5 and grad(nws=64) == -5 and grad(ws=p + 8) == -4
 
 
+@pytest.mark.parametrize("how", [{"tokens": 1 << 30}, {"tokens": (1 << 31) - 1}, {"hq": 1 << 30}, {"hk": (1 << 31) - 1}])
+def test_more_rows_than_32_bits_count_are_refused(lib, how):
+    """Tokens rounded up to a block's share, and the heads of both tensors, stay below 2^31."""
+    l = lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 63) & ~63
+    a = {"tokens": 1, "hq": 1, "hk": 1} | how
+    s8, s12 = (ctypes.c_longlong * 8)(), (ctypes.c_longlong * 12)()
+    assert l.b200ht_rotary_qk(p, p, p, p, None, None, 1e-6, a["tokens"], a["hq"], a["hk"], 64, s8, lib.BF16, p, 0, 1, 1, None, p, 32,
+                              0, None) == -2
+    assert l.b200ht_norm_rotary_qk_backward(p, p, p, p, p, p, 1e-6, p, p, p, p, a["tokens"], a["hq"], a["hk"], 64, s12, lib.BF16, p,
+                                            0, 1, 1, None, p, 32, 0, p, 1 << 30, None) == -2
+
+
 # --------------------------------------------------------------------------------------------------------- on the GPU
 SHAPES = [
     # T, q heads, k heads, D, pairs
