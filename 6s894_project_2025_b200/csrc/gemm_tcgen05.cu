@@ -21,7 +21,8 @@
 // tile's 256 tokens: its B matrix (128 * MT rows x rank) against the tokens' low-rank vectors S (256 x rank), into the
 // same accumulator, so the adapters cost rank / K of the contraction, no pass over C, and no second rounding.  The
 // instructions cover the groups of 16 tokens that have a token of the adapter; the tokens of other adapters in these
-// groups are zeroed in shared memory by the MMA warp between the copy and the instructions.
+// groups are zeroed in shared memory by the MMA warp between the copy and the instructions; what an infinity or NaN in an
+// adapter makes of these zeros is mended in the epilogue (lora_unspoilt).
 #include <cstdlib>
 #include <mutex>
 
@@ -143,6 +144,21 @@ template <bool ADAPT>
 struct AdaptArgs {};
 template <>
 struct AdaptArgs<true> : LoraOperands {};
+
+// 32 columns of the accumulator from `taddr` on: tokens n .. n + 31 of this lane's row m.
+template <bool ADAPT>
+__device__ __forceinline__ void tc_load_chunk(uint32_t (&r)[32], uint32_t taddr, int m, int n, const AdaptArgs<ADAPT> &adapt)
+{
+    tmem_ld32(taddr, r);
+    tmem_ld_wait();
+    if constexpr (ADAPT) {
+        if (!__all_sync(0xffffffffu, all_finite(r))) {
+            lora_unspoil_columns(adapt, taddr, m, n);
+            tmem_ld32(taddr, r);
+            tmem_ld_wait();
+        }
+    }
+}
 
 template <int OUT_DT, int LAYOUT, int MT, bool ADAPT>
 __global__ void __launch_bounds__(TcCfg<MT>::THREADS, 1)
@@ -350,9 +366,14 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
 #pragma unroll 1
                 for (int c = 0; c < TC_BN; c += COLS) {
                     uint32_t r[32], r2[32];
-                    tmem_ld32(taddr + c, r);
-                    if (OUT_DT != B200HT_F32) tmem_ld32(taddr + c + 32, r2);
-                    tmem_ld_wait();
+                    if constexpr (ADAPT) {
+                        tc_load_chunk<ADAPT>(r, taddr + c, m, n0 + c, adapt);
+                        if (OUT_DT != B200HT_F32) tc_load_chunk<ADAPT>(r2, taddr + c + 32, m, n0 + c + 32, adapt);
+                    } else {
+                        tmem_ld32(taddr + c, r);
+                        if (OUT_DT != B200HT_F32) tmem_ld32(taddr + c + 32, r2);
+                        tmem_ld_wait();
+                    }
                     tc_scale_chunk(r, rs, tok_scale, n0 + c, N);
                     if (OUT_DT != B200HT_F32) tc_scale_chunk(r2, rs, tok_scale, n0 + c + 32, N);
                     // the buffer about to be overwritten must have been read by its previous store
@@ -422,6 +443,14 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
                         col[(2 * j) * 128] = (unsigned short)(pk[cc * 16 + j] & 0xffffu);
                         col[(2 * j + 1) * 128] = (unsigned short)(pk[cc * 16 + j] >> 16);
                     }
+                    if constexpr (ADAPT) {
+                        const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+                        __nv_bfloat162 z = zero;   // NaN in a half once a value of that half is not finite
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) z = __hfma2(reinterpret_cast<const __nv_bfloat162 &>(pk[cc * 16 + j]), zero, z);
+                        if (!__all_sync(0xffffffffu, __hbeq2(z, zero)))
+                            lora_unspoil_staged(adapt, (__nv_bfloat16 *)col, 128, m, n0 + cc * 32);
+                    }
                     asm volatile("bar.sync %0, 128;\n" ::"r"(bar_id) : "memory");
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -434,8 +463,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
 #pragma unroll 1
                 for (int c = 0; c < TC_BN; c += 32) {
                     uint32_t r[32];
-                    tmem_ld32(taddr + c, r);
-                    tmem_ld_wait();
+                    tc_load_chunk<ADAPT>(r, taddr + c, m, n0 + c, adapt);
                     tc_scale_chunk(r, rs, tok_scale, n0 + c, N);
                     tc_store_chunk<OUT_DT, LAYOUT>(C, M, N, ldc, m, n0 + c, r);
                 }
@@ -614,16 +642,22 @@ int encode_tmap_bf16_stack(CUtensorMap *map, const void *base, uint64_t d2, uint
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-// The operands of a contraction with adapters: B in boxes of `rows` rows, S of `tokens` tokens in boxes of `box` tokens.
-int lora_operands(LoraOperands *o, const LoraGemm &lora, int tokens, int rows, int box)
+// The operands of a contraction with adapters: B in boxes of `rows` rows, S of N tokens in boxes of `box` tokens.
+int lora_operands(LoraOperands *o, const LoraGemm &lora, const void *W, const void *Y, int M, int N, int K, int rows, int box)
 {
     int rc = encode_tmap_bf16_stack(&o->tmB, lora.B, (uint64_t)lora.adapters, (uint64_t)lora.M, (uint64_t)lora.rank, (uint32_t)rows);
     if (rc) return rc;
-    rc = encode_tmap_bf16_stack(&o->tmS, lora.S, 1, (uint64_t)tokens, (uint64_t)lora.rank, (uint32_t)box,
+    rc = encode_tmap_bf16_stack(&o->tmS, lora.S, 1, (uint64_t)N, (uint64_t)lora.rank, (uint32_t)box,
                                 (uint64_t)lora_pitch(lora.rank));
     o->tiles = lora.tiles;
     o->rank = lora.rank;
     o->row = lora.row;
+    o->W = (const __nv_bfloat16 *)W;
+    o->Y = (const __nv_bfloat16 *)Y;
+    o->B = (const __nv_bfloat16 *)lora.B;
+    o->S = (const __nv_bfloat16 *)lora.S;
+    o->index = lora.index;
+    o->K = K, o->M = M, o->N = N, o->rows_b = lora.M, o->adapters = lora.adapters;
     return rc;
 }
 
@@ -667,7 +701,7 @@ static int launch_tc_mt(const void *Y, const void *W, void *C, int M, int N, int
     const int grid = tiles < sm_count() ? tiles : sm_count();
     if (lora) {
         AdaptArgs<true> ad{};
-        rc = lora_operands(&ad, *lora, N, Cfg::BM, TC_BN);
+        rc = lora_operands(&ad, *lora, W, Y, M, N, K, Cfg::BM, TC_BN);
         if (rc) return rc;
         rc = ensure_dyn_smem((const void *)gemm_tc_kernel<OUT_DT, LAYOUT, MT, true>, Cfg::SMEM_BYTES);
         if (rc) return rc;

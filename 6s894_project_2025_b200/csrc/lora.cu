@@ -775,7 +775,7 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     rc = shrink_by_rows(N, K, rank) ? launch_shrink_rows(X, A, index, scaling, S, N, K, adapters, rank, 1, true, st)
                                     : launch_shrink_tiles(X, A, index, scaling, S, N, K, adapters, rank, st);
     if (rc) return rc;
-    const LoraGemm lora{B, S, tiles, adapters, M, rank, 0};
+    const LoraGemm lora{B, S, tiles, index, adapters, M, rank, 0};
     return fused_gemm_bf16_lora(X, W, C, M, N, K, out_dtype, out_layout, scale, signs, workspace, st, lora);
 }
 

@@ -19,6 +19,7 @@ struct LoraGemm {
     const void *B;       // [adapters][M][rank] bf16
     const void *S;       // [tokens][lora_pitch(rank)] bf16, rank of each used: scaling * A x of each token's adapter, 0 without one
     const int *tiles;    // kLoraTileInts per 256-token tile
+    const int *index;    // adapter of each token
     int adapters, M, rank;
     int row;             // row of B that belongs to the first row of C
 
@@ -29,6 +30,7 @@ struct LoraGemm {
         o.row += (int)r;
         o.S = (const unsigned char *)S + (size_t)t * lora_pitch(rank) * 2;
         o.tiles = tiles + (size_t)(t / 256) * kLoraTileInts;
+        o.index = index + t;
         return o;
     }
 };

@@ -178,7 +178,13 @@ lora_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
         for (int p = 0; p < 8; ++p)
             if (p < split) sum = make_float4(sum.x + v[p].x, sum.y + v[p].y, sum.z + v[p].z, sum.w + v[p].w);
         const int m = m0 + 4 * lane;
-        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (isnan(f[0]) || isnan(f[1]) || isnan(f[2]) || isnan(f[3])) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (m + e < M && isnan(f[e])) f[e] = lora_unspoilt(lora, m + e, n0 + t, f[e]);
+            sum = make_float4(f[0], f[1], f[2], f[3]);
+        }
         if (LAYOUT == B200HT_OUT_NM && (M & 3) == 0) {
             const size_t i = (size_t)(n0 + t) * M + m;
             if (m < M) {
@@ -224,7 +230,7 @@ static int launch_split(const void *Y, const void *W, void *C, int M, int N, int
     rc = encode_tmap_bf16_2d(&ty, Y, (uint64_t)N, (uint64_t)K, (uint32_t)box);
     if (rc) return rc;
     LoraOperands o{};
-    rc = lora_operands(&o, lora, N, 128, box);
+    rc = lora_operands(&o, lora, W, Y, M, N, K, 128, box);
     if (rc) return rc;
     constexpr int smem = kSplitRing + 1024 + 256;
     rc = ensure_dyn_smem((const void *)lora_gemm_split_kernel<OUT_DT, LAYOUT>, smem);

@@ -74,8 +74,9 @@ def lora_ht_gemm(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Ten
     transform and do not touch the adapters.  Tokens may come in any order; tokens of one adapter next to each other cost
     least.  The low-rank vectors are rounded to bf16, as H(X) is, the sums are fp32 and C is rounded once.
 
-    An adapter's B is multiplied with zeros for the other tokens of a group of 16 (tokens 16 i .. 16 i + 15) that has one
-    of its own: its values must be finite.  Adapters that no token names are not read.
+    Infinities and NaN in an adapter reach its own tokens only; a call with such an adapter among others in a group of 16
+    tokens (16 i .. 16 i + 15) is much slower, as these results are computed again.  Adapters that no token names are not
+    read.
     """
     if X.dim() != 2 or W.dim() != 2 or X.shape[1] != W.shape[1]:
         raise RuntimeError("lora_ht_gemm: expected X (N, K) and W (M, K)")

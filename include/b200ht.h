@@ -289,8 +289,9 @@ int b200ht_norm_rotary_qk_backward(const void *dq_out, const void *dk_out, const
  *   signs    as in b200ht_fused_gemm_signed, or NULL
  * K a power of two, 64 .. 32768; rank a multiple of 8, 8 .. 128 (pad with rows and columns of zeros).  W, X, A, B bf16;
  * H(X) (fp32 throughout here) and the low-rank vectors are rounded to bf16 once, everything else is accumulated in fp32.
- * An adapter's B is multiplied with zeros for the other tokens of a group of 16 (tokens 16 i .. 16 i + 15) that has one
- * of its tokens: infinities or NaN in B reach those tokens too.  Adapters that no token names are not read.
+ * Infinities and NaN in an adapter reach its own tokens only; with such an adapter among others in a group of 16 tokens
+ * (16 i .. 16 i + 15) the call is much slower, as these results are computed again.  Adapters that no token names are not
+ * read.
  * `workspace`: b200ht_lora_gemm_workspace_bytes(M, N, K, rank) bytes, 256-byte aligned.  Calls that share one must not
  * run at the same time.
  */

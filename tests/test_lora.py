@@ -461,3 +461,70 @@ def test_results_beyond_32_bits(pkg):
     want = small.double().cpu()
     off = (got[last].double().cpu() - want).abs()
     assert bool((off <= room + (want.abs() + room) * 2.0 ** -8).all())
+
+
+BROKEN = [
+    # tokens, K, M, rank, adapters, M x N layout, result: the clusters' kernel, tiles of 128 and 256 rows, a tail of 128-row
+    # tiles behind 256-row ones, tokens in chunks; the three ways a tile's results leave
+    (40, 256, 140, 16, 6, "nm", torch.float32), (40, 256, 130, 16, 6, "mn", torch.bfloat16), (300, 512, 257, 128, 5, "nm", torch.bfloat16),
+    (1500, 256, 4096, 72, 7, "mn", torch.float32), (1504, 256, 4096, 24, 7, "mn", torch.bfloat16), (1500, 256, 4096, 8, 7, "nm", torch.bfloat16),
+    (3000, 64, 4096, 16, 5, "nm", torch.bfloat16), (3000, 64, 4100, 16, 5, "mn", torch.float32), (1600, 16384, 64, 16, 4, "nm", torch.float32),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", BROKEN, ids=lambda s: "x".join(map(str, s[:5])) + s[5])
+@pytest.mark.parametrize("how", ["all", "one"])
+def test_a_broken_adapter_stays_with_its_tokens(pkg, shape, how):
+    """Infinities and NaN in an adapter that tokens do use: the others, beside them in every tile, keep their results.
+
+    Both calls have the same H(X) and S, bit for bit.  Where a result is computed again, the two differ by their sums: on the
+    tensor cores K / 16 + rank / 16 + 1 additions off by at most 2^-22 each of the sum of the products' sizes; in fp32 K / 8
+    + rank / 8 + 3 additions off by 2^-24.  The sizes take the rounding of H(X) and S to bf16 along, 1 + 2^-8."""
+    N, K, M, R, L, layout, dtype = shape
+    X, W, A, B, index, scaling = make(N, K, M, R, L, seed=21, spread="any")
+    index[N // 2:N // 2 + 40] = 1      # whole groups of other adapters, and of the broken one
+    index[N // 4:N // 4 + 20] = 2
+    broken = B.clone()
+    rows = torch.arange(M)
+    if how == "all":
+        broken[2] = float("inf")
+        hit = rows >= 0
+    else:
+        broken[2, 0, 3] = float("nan")
+        broken[2, M - 1, 7] = float("-inf")
+        hit = (rows == 0) | (rows == M - 1)
+
+    def call(b, out_dtype):
+        y = pkg.lora_ht_gemm(X, W, A, b, index, scaling=scaling, out_layout=layout, out_dtype=out_dtype)
+        return (y if layout == "nm" else y.t()).cpu()
+
+    clean, got = call(B, torch.float32), call(broken, torch.float32)
+    assert pkg.device_status() == 0
+    mine = index.cpu() == 2
+    assert torch.equal(got[:, ~hit], clean[:, ~hit])
+    assert not torch.isfinite(got[mine][:, hit]).any()
+    if how == "one":
+        assert torch.isnan(got[mine, 0]).all()
+        S = (X[mine.cuda()].double() @ A[2, 7].double() * scaling[2].double()).cpu()
+        sure = S.abs() > 1e-3          # the sign of an element far from zero
+        assert bool(sure.any()) and torch.equal(got[mine, M - 1][sure], -torch.sign(S[sure]).float() * float("inf"))
+    _, _, share = share64(X, A, B, index, scaling)
+    x, h, n = X.double().cpu(), X.double().cpu(), 1
+    while n < K:
+        h = h.reshape(-1, K // (2 * n), 2, n)
+        h = torch.stack([h[:, :, 0] + h[:, :, 1], h[:, :, 0] - h[:, :, 1]], 2).reshape(-1, K)
+        n *= 2
+    size = ((h * K ** -0.5).abs() @ W.double().cpu().abs().t() + share) * (1 + 2.0 ** -8)
+    allowed = size * ((K / 16 + R / 16 + 1) * 2.0 ** -22 + (K / 8 + R / 8 + 3) * U)
+    off = (got.double() - clean.double()).abs()[~mine]
+    assert bool((off <= allowed[~mine]).all())
+    if dtype == torch.bfloat16:
+        assert torch.equal(call(broken, dtype)[~mine], got.bfloat16()[~mine])
+    # a token's own NaN among them
+    X[N // 4 + 3, 5] = float("nan")
+    again = call(broken, torch.float32)
+    assert torch.isnan(again[N // 4 + 3]).all()
+    others = ~mine
+    others[N // 4 + 3] = False
+    assert torch.equal(again[others], got[others])
