@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DT, _is_pow2, _on_device, _stream_ptr
+from .ops import _DT, _check_overwrite, _is_pow2, _on_device, _overwritten, _stream_ptr
 
 _INTS = (torch.int32, torch.int64)
 _strides8 = struct.Struct("8q").pack
@@ -149,6 +149,9 @@ def _run(q, k, q_weight, k_weight, eps, positions, inv_freq, sections, axis_orde
     if inplace:
         if q is not q_in or k is not k_in:
             raise RuntimeError("rotary: the last dimension must be contiguous to work in place")
+        _check_overwrite("rotary", q)
+        if k is not None:
+            _check_overwrite("rotary", k)
         if not _own_memory(q) or (k is not None and not (_own_memory(k) and _apart(q, k))):
             raise RuntimeError("rotary: in place, queries and keys must not share memory with themselves or each other")
         qo, ko = q, k
@@ -171,6 +174,10 @@ def _run(q, k, q_weight, k_weight, eps, positions, inv_freq, sections, axis_orde
                 _DT[q.dtype], positions.data_ptr(), pa, pt, n_axes, table, inv_freq.data_ptr(), pairs, flags,
                 _stream_ptr(q.device))
         _lib.check(rc, "b200ht_rotary_qk")
+        if inplace:
+            _overwritten(q)
+            if k is not None:
+                _overwritten(k)
     return qo, ko
 
 
@@ -189,7 +196,8 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
 
     ``hadamard`` multiplies every rotated head by H / sqrt(head_dim) (Sylvester order, as ``hadamard_transform``).
     ``inverse`` undoes the call without it, which is also its gradient: H first, then the rotation by the negative
-    angles.  ``inplace`` overwrites q and k and returns them; tensors that overlap themselves or each other are refused.
+    angles.  ``inplace`` overwrites q and k and returns them; tensors that overlap themselves or each other are refused, and
+    while a graph is recorded those that require grad.
     """
     return _run(q, k, None, None, 0.0, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse, inplace)
 

@@ -45,6 +45,18 @@ def _on_device(device: torch.device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _check_overwrite(what: str, x: torch.Tensor) -> None:
+    """Refuse a tensor of a graph that is being recorded: the graph would not see its values replaced."""
+    if torch.is_grad_enabled() and (x.requires_grad or (x._base is not None and x._base.requires_grad)):
+        raise RuntimeError(f"{what}: a tensor that requires grad cannot be overwritten (wrap the call in torch.no_grad())")
+
+
+def _overwritten(x: torch.Tensor) -> None:
+    """Tell autograd that x has new values, so that a backward that saved the old ones fails instead of using the new."""
+    if not x.is_inference():   # these have no version
+        torch.autograd.graph.increment_version(x)
+
+
 def sign_mask(signs: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
     """+-1 diagonal (length n, any real dtype) -> the 16-bit sign-bit table the library takes
     (0x8000 where the entry is negative), padded to a whole 16-byte vector."""

@@ -164,6 +164,37 @@ def test_shared_memory_of_one_expanded_token_is_found(pkg):
     assert not heads._apart(x[:, :4], x[:, 3:]) and not heads._apart(x[:, 3:], x[:, :4])
 
 
+def test_tensors_of_a_graph_are_not_overwritten(pkg):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        p, f, w = t(5, dtype=torch.int64), t(32, dtype=torch.float32), t(64)
+        q, k, leaf = t(5, 4, 64), t(5, 2, 64), t(5, 6, 64).requires_grad_()
+        with torch.no_grad():
+            view = leaf[:, :4]
+        for bq, bk in [(t(5, 4, 64).requires_grad_(), k), (q, t(5, 2, 64).requires_grad_()), (leaf[:, :4], k), (view, None)]:
+            with pytest.raises(RuntimeError, match="requires grad"):
+                pkg.rotary_qk(bq, bk, p, f, inplace=True)
+        with pytest.raises(RuntimeError, match="requires grad"):
+            pkg.norm_rotary_qk(leaf[:, :4], leaf[:, 4:], w, w, p, f, inplace=True)
+
+
+def test_overwriting_counts_as_a_new_version(pkg):
+    import importlib
+    ops = importlib.import_module("6s894_project_2025_b200.ops")
+    x = torch.zeros(4, 6)
+    before = x._version
+    ops._overwritten(x[:, :3])
+    assert x._version > before and x.detach()._version == x._version
+    with torch.inference_mode():
+        y = torch.zeros(3)
+        ops._overwritten(y)
+    ops._overwritten(y)   # an inference tensor has no version, inside the mode or outside
+
+
 def test_c_entries_refuse_before_the_gpu(lib):
     l = lib.load()
     buf = ctypes.create_string_buffer(4096)
@@ -537,3 +568,27 @@ def test_gradients_captured_in_a_graph(pkg):
     want = pkg.norm_rotary_qk_backward(dq, dk, q.flip(0), k, w, w, pos, inv, hadamard=True)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_backward_that_saved_what_was_overwritten_fails(pkg):
+    """q and k are views of a projection that another operation has saved: its backward must not use the rotated values."""
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    q, k, pos, inv = make(7, 4, 2, 64, 32, torch.bfloat16, packed=True, far=50)
+    scale = torch.ones(1, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    for call in (lambda: pkg.rotary_qk(q, None, pos, inv, inplace=True), lambda: pkg.rotary_qk(k, q, pos, inv, inplace=True),
+                 lambda: pkg.norm_rotary_qk(q, k, w, w, pos, inv, inplace=True)):
+        y = (q._base * scale).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    y = (q._base * scale).sum()
+    pkg.rotary_qk(q, k, pos, inv)
+    y.backward()          # not in place: nothing was overwritten
+    leaf = q.float().bfloat16().requires_grad_()
+    with torch.no_grad():
+        assert pkg.rotary_qk(leaf, None, pos, inv, inplace=True)[0] is leaf
+    with torch.inference_mode():
+        cache = q.clone()
+        pkg.rotary_qk(cache, None, pos, inv, inplace=True)
+    pkg.rotary_qk(cache, None, pos, inv, inplace=True)
