@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _DT, _is_pow2, _on_device, _stream_ptr, sign_mask
+from .ops import _DT, _check_overwrite, _is_pow2, _on_device, _overwritten, _stream_ptr, sign_mask
 
 _MAX_COLUMNS = 64   # columns of one decoding call; more go through the contraction
 
@@ -59,6 +59,8 @@ def _out(what, out, shape, dtype, like):
         return like.new_empty(shape, dtype=dtype)
     if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.device != like.device or out.data_ptr() % 16:
         raise RuntimeError(f"{what}: out has the wrong shape, dtype, strides, device or alignment")
+    _check_overwrite(what, out)
+    _overwritten(out)
     return out
 
 

@@ -131,6 +131,20 @@ def test_refusals_of_the_python_entries(pkg):
                 pkg.lora_ht_gemv(**{**columns, **change})
 
 
+def test_an_output_of_a_graph_is_not_overwritten(pkg):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        X, W, A, B, index = t(20, 128), t(48, 128), t(3, 16, 128), t(3, 48, 16), t(20, dtype=torch.int32)
+        with pytest.raises(RuntimeError, match="requires grad"):
+            pkg.lora_ht_gemm(X, W, A, B, index, out=t(48, 20, dtype=torch.float32).requires_grad_())
+        with pytest.raises(RuntimeError, match="requires grad"):
+            pkg.lora_ht_gemv(W, t(128, 8), A, B, index[:8], out=t(48, 8, dtype=torch.float32).requires_grad_())
+
+
 def test_c_entries_refuse_before_the_gpu(lib):
     l = lib.load()
     buf = ctypes.create_string_buffer(4096)
@@ -528,3 +542,17 @@ def test_a_broken_adapter_stays_with_its_tokens(pkg, shape, how):
     others = ~mine
     others[N // 4 + 3] = False
     assert torch.equal(again[others], got[others])
+
+
+@pytest.mark.gpu
+def test_a_backward_that_saved_an_output_fails_once_it_is_overwritten(pkg):
+    X, W, A, B, index, scaling = make(33, 256, 48, 16, 3, seed=22)
+    scale = torch.ones(1, device="cuda", requires_grad=True)
+    Xc, some = X[:4].t().contiguous(), index[:4].contiguous()
+    for shape, call in (((33, 48), lambda out: pkg.lora_ht_gemm(X, W, A, B, index, out_layout="nm", out=out)),
+                        ((48, 4), lambda out: pkg.lora_ht_gemv(W, Xc, A, B, some, out=out))):
+        out = torch.randn(shape, device="cuda")
+        y = (out * scale).sum()
+        assert call(out) is out and torch.equal(out, call(torch.empty(shape, device="cuda")))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
