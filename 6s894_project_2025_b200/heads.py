@@ -94,6 +94,8 @@ def _check_common(q, positions, inv_freq, sections, axis_order, hadamard):
 
 
 def _check_weights(q, q_weight, k_weight, D):
+    if q_weight is None or k_weight is None:
+        raise RuntimeError("norm_rotary_qk: both weights are required, also without keys (any vector like q_weight will do)")
     device, dtype = q.device, q_weight.dtype
     for w in (q_weight, k_weight):
         if tuple(w.shape) != (D,) or w.device != device:
@@ -134,14 +136,14 @@ def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
     return at >= reach(q[0]) and at + reach(k[0]) <= row
 
 
-def _run(q, k, q_weight, k_weight, eps, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse, inplace):
+def _run(q, k, norm, q_weight, k_weight, eps, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse, inplace):
     D, tokens, pairs, flags, table, n_axes, pa, pt = _check_common(q, positions, inv_freq, sections, axis_order, hadamard)
     q_in, k_in = q, k
     if q.stride(2) != 1:
         q = q.contiguous()
     if k is not None:
         k = _check_heads(k, q, "keys")
-    if q_weight is not None:
+    if norm:
         _check_weights(q, q_weight, k_weight, D)
         q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
         if q_weight.dtype == torch.float32:
@@ -199,19 +201,20 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
     angles.  ``inplace`` overwrites q and k and returns them; tensors that overlap themselves or each other are refused, and
     while a graph is recorded those that require grad.
     """
-    return _run(q, k, None, None, 0.0, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse, inplace)
+    return _run(q, k, False, None, None, 0.0, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse, inplace)
 
 
-def norm_rotary_qk(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+def norm_rotary_qk(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor, k_weight: torch.Tensor,
                    positions: torch.Tensor, inv_freq: torch.Tensor, *, eps: float = 1e-6,
                    sections: tuple[int, ...] | None = None, axis_order: str = "blocks", interleaved: bool = False,
                    hadamard: bool = False, inplace: bool = False):
     """``rotary_qk`` behind an RMS norm of every head: ``x * rsqrt(mean(x^2) + eps) * weight``, one pass, one rounding.
 
     ``q_weight`` and ``k_weight`` (head_dim entries) both have the queries' dtype, or both are float32.  Everything else
-    as :func:`rotary_qk`; the gradients are :func:`norm_rotary_qk_backward`.
+    as :func:`rotary_qk` (without keys both weights are needed all the same); the gradients are
+    :func:`norm_rotary_qk_backward`.
     """
-    return _run(q, k, q_weight, k_weight, float(eps), positions, inv_freq, sections, axis_order, interleaved, hadamard,
+    return _run(q, k, True, q_weight, k_weight, float(eps), positions, inv_freq, sections, axis_order, interleaved, hadamard,
                 False, inplace)
 
 
@@ -222,10 +225,12 @@ def norm_rotary_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
     """Gradients of :func:`norm_rotary_qk`: returns ``(dq, dk, dq_weight, dk_weight)``.
 
     ``dq_out`` and ``dk_out`` are the gradients of its results, the other arguments those of the call (``q`` and ``k``
-    before it: a call in place has lost them).  The weights' gradients are sums over all tokens and heads, in fp32 and
+    before it: a call in place has lost them).  Without keys pass tensors of none, ``q[:, :0]``.  The weights' gradients are sums over all tokens and heads, in fp32 and
     in an order that depends on the sizes alone.
     """
     D, tokens, pairs, flags, table, n_axes, pa, pt = _check_common(q, positions, inv_freq, sections, axis_order, hadamard)
+    if k is None or dk_out is None:
+        raise RuntimeError("norm_rotary_qk_backward: keys and their gradients are required; without keys pass q[:, :0] for both")
     k = _check_heads(k, q, "keys")
     if q.stride(2) != 1:
         q = q.contiguous()

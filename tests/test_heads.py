@@ -164,6 +164,24 @@ def test_shared_memory_of_one_expanded_token_is_found(pkg):
     assert not heads._apart(x[:, :4], x[:, 3:]) and not heads._apart(x[:, 3:], x[:, :4])
 
 
+def test_missing_keys_and_weights_are_named(pkg):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        q, k, p, f, w = t(5, 4, 64), t(5, 2, 64), t(5, dtype=torch.int64), t(32, dtype=torch.float32), t(64)
+        for bk, qw, kw in [(None, w, None), (k, w, None), (k, None, w), (None, None, None)]:
+            with pytest.raises(RuntimeError, match="both weights are required"):
+                pkg.norm_rotary_qk(q, bk, qw, kw, p, f)
+            with pytest.raises(RuntimeError, match="required"):
+                pkg.norm_rotary_qk_backward(q, k, q, bk, qw, kw, p, f)
+        for dk, bk in [(None, k), (k, None), (None, None)]:
+            with pytest.raises(RuntimeError, match="keys and their gradients"):
+                pkg.norm_rotary_qk_backward(q, dk, q, bk, w, w, p, f)
+
+
 def test_tensors_of_a_graph_are_not_overwritten(pkg):
     from torch._subclasses.fake_tensor import FakeTensorMode
 
@@ -592,3 +610,17 @@ def test_a_backward_that_saved_what_was_overwritten_fails(pkg):
         cache = q.clone()
         pkg.rotary_qk(cache, None, pos, inv, inplace=True)
     pkg.rotary_qk(cache, None, pos, inv, inplace=True)
+
+
+@pytest.mark.gpu
+def test_norm_without_keys(pkg):
+    """None for the keys, or keys of no head, forward; keys of no head backward."""
+    q, _, pos, inv = make(9, 4, 0, 64, 32, torch.bfloat16, far=40)
+    w = torch.linspace(0.5, 1.5, 64, device="cuda").bfloat16()
+    y, none = pkg.norm_rotary_qk(q, None, w, w, pos, inv, hadamard=True)
+    assert none is None
+    assert_close(y, forward64(q, w, 1e-6, pos, inv, hadamard=True))
+    assert torch.equal(pkg.norm_rotary_qk(q, q[:, :0], w, w, pos, inv, hadamard=True)[0], y)
+    with_keys = pkg.norm_rotary_qk_backward(q, q, q, q, w, w, pos, inv)
+    without = pkg.norm_rotary_qk_backward(q, q[:, :0], q, q[:, :0], w, w, pos, inv)
+    assert torch.equal(without[0], with_keys[0]) and without[1].shape == (9, 0, 64) and not without[3].any()
