@@ -17,6 +17,11 @@ from . import _lib
 from .ops import _DT, _check_overwrite, _is_pow2, _on_device, _overwritten, _stream_ptr, sign_mask
 
 _MAX_COLUMNS = 64   # columns of one decoding call; more go through the contraction
+# Beyond N = 8192 the GEMV takes four columns a pass over W (one at 32768), the contraction all.  Microseconds a call, GEMV
+# and contraction, 16384 x 16384: 3 columns 184 / 207, 4: 255 / 119, 16: 991 / 129, 64: 4599 / 138; M = 4096, N = 16384: 3
+# columns 95 / 43, 4: 128 / 43; N = 32768: 3 columns 416 / 71, 64: 9883 / 109.  Up to three columns W . H(X) keeps the bits
+# of fused_ht_gemv.
+_LONG, _LONG_COLUMNS = 8192, 3
 
 
 def _check(what: str, X, W, A, B, index, scaling, tokens: int, K: int, out_dtype):
@@ -113,7 +118,8 @@ def lora_ht_gemv(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Ten
     ``W`` is (M, N), ``X`` (N, columns) with the columns fastest (or a vector, one column), the result (M, columns);
     ``A`` (adapters, rank, N), ``B`` (adapters, M, rank), ``index`` (columns int32 entries) and ``scaling`` as in
     :func:`lora_ht_gemm`.  The low-rank vectors stay fp32 and Y is rounded once.  Beyond the batch that
-    ``fused_ht_gemv`` serves with one pass over W the call goes through :func:`lora_ht_gemm`.
+    ``fused_ht_gemv`` serves with one pass over W (16 columns at N = 4096; three for N above 8192, which are a pass at 16384
+    and three at 32768) the call goes through :func:`lora_ht_gemm`.
     """
     if X.dim() == 1:
         X = X[:, None]
@@ -125,7 +131,7 @@ def lora_ht_gemv(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Ten
     out_dtype = out_dtype or torch.float32
     lib = _lib.load()
     once = lib.b200ht_fused_gemv_max_batch(N, _lib.BF16)   # columns served by one pass over W
-    if columns > _MAX_COLUMNS or (once and columns > once):
+    if columns > _MAX_COLUMNS or (once and columns > once) or (N > _LONG and columns > _LONG_COLUMNS):
         return lora_ht_gemm(X.t(), W, A, B, index, scaling=scaling, scale=scale, out_dtype=out_dtype, out=out)
     M, adapters, rank, A, B, index, scaling = _check("lora_ht_gemv", X, W, A, B, index, scaling, columns, N, out_dtype)
     X, W = _rows(X), _rows(W)

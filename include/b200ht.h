@@ -304,6 +304,9 @@ int b200ht_lora_gemm(const void *X, const void *W, void *C, const void *A, const
  * The same for a decoding batch, in the layouts of b200ht_fused_gemv (bf16): X  N x B with b fastest, Y  M x B with b
  * fastest, index[b] the adapter of column b, 1 <= B <= 64, N a power of two, 64 .. 32768.  The low-rank vectors stay
  * fp32; one rounding.  `workspace`: b200ht_lora_gemv_workspace_bytes(M, N, B, rank) bytes, 256-byte aligned.
+ * W is read once for up to b200ht_fused_gemv_max_batch(N) columns (256 <= N <= 8192), or 64 (N <= 128); more columns take
+ * a pass for each such group, four columns a pass at N = 16384, one at 32768.  b200ht_lora_gemm reads W once for all and is
+ * the faster entry there (the tokens lie one behind the other then).
  */
 size_t b200ht_lora_gemv_workspace_bytes(int M, int N, int B, int rank);
 int b200ht_lora_gemv(const void *W, const void *X, void *Y, const void *A, const void *Bm, const int *index,

@@ -270,6 +270,20 @@ def test_decoding_beyond_one_pass_over_the_weight(pkg, columns):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [16384, 32768])
+@pytest.mark.parametrize("columns", [4, 5, 17, 64])
+def test_decoding_with_long_columns_reads_the_weight_once(pkg, columns, N):
+    """The GEMV would read W for every fourth column, or for each: the call has to be the contraction's."""
+    X, W, A, B, index, scaling = make(columns, N, 72, 16, 3, seed=columns, spread="any")
+    base = pkg.lora_ht_gemv(W, X.t().contiguous(), A, B, torch.full_like(index, -1))
+    got = pkg.lora_ht_gemv(W, X.t().contiguous(), A, B, index, scaling=scaling)
+    assert got.shape == (72, columns)
+    assert torch.equal(got, pkg.lora_ht_gemm(X, W, A, B, index, scaling=scaling))
+    check_base(base.t(), X, W)
+    check_share(got.t(), base.t(), X, A, B, index, scaling)
+
+
+@pytest.mark.gpu
 def test_a_vector_is_one_column(pkg):
     X, W, A, B, index, scaling = make(1, 1024, 50, 8, 2, spread="1")
     assert torch.equal(pkg.lora_ht_gemv(W, X[0], A, B, index), pkg.lora_ht_gemv(W, X.t().contiguous(), A, B, index))
