@@ -411,7 +411,8 @@ __device__ __forceinline__ void row_turn(RowTurn &t, const float2 *tab, int mode
     }
 }
 
-__device__ __forceinline__ void row_rotate(float2 (&v)[2][4], const RowTurn &t, int mode, int partner)
+// Dimensions behind the pairs are not touched: times 1 and 0, an infinity among them would be NaN and reach its neighbour.
+__device__ __forceinline__ void row_rotate(float2 (&v)[2][4], const RowTurn &t, int mode, int partner, int j, int D, int pairs)
 {
     if (mode == kPairsHalves) {
 #pragma unroll
@@ -421,20 +422,26 @@ __device__ __forceinline__ void row_rotate(float2 (&v)[2][4], const RowTurn &t, 
             v[1][i] = fma2(b, t.c[i], mul2(a, t.s[i]));
         }
     } else if (mode == kPairsNeighbour) {
+        const auto turn = [&](int s, int i) {
+            const float c = i & 1 ? t.c[2 * s + (i >> 1)].y : t.c[2 * s + (i >> 1)].x;
+            const float sn = i & 1 ? t.s[2 * s + (i >> 1)].y : t.s[2 * s + (i >> 1)].x;
+            const float a = v[s][i].x, b = v[s][i].y;
+            v[s][i] = make_float2(a * c - b * sn, b * c + a * sn);
+        };
+        if (2 * pairs == D) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+            for (int i = 0; i < 8; ++i) turn(i >> 2, i & 3);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float c = i & 1 ? t.c[2 * s + (i >> 1)].y : t.c[2 * s + (i >> 1)].x;
-                const float sn = i & 1 ? t.s[2 * s + (i >> 1)].y : t.s[2 * s + (i >> 1)].x;
-                const float a = v[s][i].x, b = v[s][i].y;
-                v[s][i] = make_float2(a * c - b * sn, b * c + a * sn);
-            }
+            for (int i = 0; i < 8; ++i)
+                if ((i >> 2) * (D / 4) + 4 * j + (i & 3) < pairs) turn(i >> 2, i & 3);
+        }
     } else {
+        const bool turns = partner != (int)(threadIdx.x & 31);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 o = make_float2(__shfl_sync(0xffffffffu, v[0][i].x, partner), __shfl_sync(0xffffffffu, v[0][i].y, partner));
-            v[0][i] = fma2(o, t.s[i], mul2(v[0][i], t.c[i]));
+            if (turns) v[0][i] = fma2(o, t.s[i], mul2(v[0][i], t.c[i]));
         }
     }
 }
@@ -553,7 +560,7 @@ rotary_row_kernel(const __grid_constant__ RotArgs a, int tb, int mode)
             scale *= rsqrtf(sum * inv_d + a.eps);
         }
         if (HAD && !NORM && a.inverse) row_hadamard<LANES>(v, j, lanes);
-        row_rotate(v, turn, mode, partner);
+        row_rotate(v, turn, mode, partner, jj, D, a.pairs);
         if (HAD && (NORM || !a.inverse)) row_hadamard<LANES>(v, j, lanes);
         if (HAD || NORM) row_scale(v, scale);
         if (on) row_store<DT>(out, half * SIZE, v);
@@ -723,7 +730,7 @@ norm_rotary_row_grad_kernel(const __grid_constant__ RotArgs a, int per_q, int pe
                     }
                 }
             } else {
-                row_rotate(g, turn, MODE, partner);
+                row_rotate(g, turn, MODE, partner, jj, D, a.pairs);
             }
             float2 q = make_float2(0.f, 0.f), d = make_float2(0.f, 0.f);
 #pragma unroll

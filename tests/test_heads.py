@@ -417,6 +417,34 @@ def test_rows_of_zeros_and_of_not_a_number(pkg):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,pairs", [(128, 32), (128, 30), (96, 24), (64, 8), (256, 64), (80, 20), (66, 20), (16, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_dimensions_behind_the_pairs_are_left_alone(pkg, D, pairs, dtype, interleaved):
+    """Infinities, NaN and the sign of a zero among them stay, and do not reach the other dimensions."""
+    q, k, pos, inv = make(40, 5, 2, D, pairs, dtype, seed=6, far=300)
+    clean = pkg.rotary_qk(q, None, pos, inv, interleaved=interleaved)[0]
+    for t, value in enumerate([float("inf"), float("-inf"), float("nan"), -0.0] * 8):
+        for h in range(5):
+            q[t, h, 2 * pairs + (t * 5 + h) % (D - 2 * pairs)] = value
+    for inverse in (False, True):
+        y = pkg.rotary_qk(q, None, pos, inv, interleaved=interleaved, inverse=inverse)[0]
+        # NaN stays NaN, with the payload that the conversion to the type gives every NaN; all else keeps its bits
+        whole = torch.int16 if dtype == torch.bfloat16 else torch.int32
+        got, want = y[..., 2 * pairs:], q[..., 2 * pairs:]
+        nan = torch.isnan(want)
+        assert torch.equal(torch.isnan(got), nan) and torch.equal(got.view(whole)[~nan], want.view(whole)[~nan])
+        assert torch.isfinite(y[..., :2 * pairs]).all()
+    assert torch.equal(pkg.rotary_qk(q, None, pos, inv, interleaved=interleaved)[0][..., :2 * pairs], clean[..., :2 * pairs])
+    # the weights' gradient is a sum over rows for each dimension: an infinite gradient stays in its own
+    w = torch.ones(D, dtype=dtype, device="cuda")
+    x, dy = torch.ones_like(q), torch.ones_like(q)
+    dy[3, 1, D - 1] = float("inf")
+    dw = pkg.norm_rotary_qk_backward(dy, dy[:, :0], x, x[:, :0], w, w, pos, inv, interleaved=interleaved)[2]
+    assert torch.isinf(dw[D - 1]) and torch.isfinite(dw[:D - 1]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("op", ["rotary", "norm"])
 def test_gradients_of_the_registered_operators(pkg, op):
     """The gradient against differences of the forward pass in fp32: along a random direction the derivative of
