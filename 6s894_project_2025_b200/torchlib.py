@@ -10,7 +10,8 @@ under the ``b200ht`` namespace:
 * ``torch.ops.b200ht.fused_ht_gemm(X, W, scale, token_major, out_bf16)``
 * ``torch.ops.b200ht.fused_ht_gemv(W, X, scale, out_bf16)``
 * ``torch.ops.b200ht.rotary_qk(q, k, positions, inv_freq, sections, axis_order, interleaved, hadamard, inverse)``
-  — autograd: the inverse call on the incoming gradients.
+  — autograd: the inverse call on the incoming gradients; a backward that needs one of inv_freq is refused, here and below.
+  Keys are required (``q[:, :0]`` without any).
 * ``torch.ops.b200ht.norm_rotary_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, axis_order,
   interleaved, hadamard)`` — autograd: gradients of q, k and both weights.
 * ``torch.ops.b200ht.lora_ht_gemm(X, W, A, B, index, scaling, scale, token_major, out_bf16)`` and
@@ -79,6 +80,11 @@ def _some(grad, x):
     return torch.zeros(x.shape, dtype=x.dtype, device=x.device) if grad is None else grad
 
 
+def _no_gradient(needed, what):
+    if needed:
+        raise RuntimeError(f"{what}: inv_freq has no gradient here; detach it")
+
+
 @torch.library.custom_op("b200ht::rotary_qk", mutates_args=(), device_types="cuda")
 def rotary_qk_op(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                  sections: Optional[Sequence[int]] = None, axis_order: str = "blocks", interleaved: bool = False,
@@ -99,6 +105,7 @@ def _rotary_setup(ctx, inputs, output):
 
 
 def _rotary_backward(ctx, dq, dk):
+    _no_gradient(ctx.needs_input_grad[3], "rotary_qk")
     positions, inv_freq = ctx.saved_tensors
     qs, ks, dtype, device = ctx.like
     dq = torch.zeros(qs, dtype=dtype, device=device) if dq is None else dq
@@ -148,6 +155,7 @@ def _norm_rotary_setup(ctx, inputs, output):
 
 
 def _norm_rotary_backward(ctx, dq, dk):
+    _no_gradient(ctx.needs_input_grad[5], "norm_rotary_qk")
     q, k, *rest = ctx.saved_tensors
     grads = torch.ops.b200ht.norm_rotary_qk_backward(_some(dq, q), _some(dk, k), q, k, *rest, *ctx.how)
     return (*grads, None, None, None, None, None, None, None)

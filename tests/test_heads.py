@@ -652,3 +652,20 @@ def test_norm_without_keys(pkg):
     with_keys = pkg.norm_rotary_qk_backward(q, q, q, q, w, w, pos, inv)
     without = pkg.norm_rotary_qk_backward(q, q[:, :0], q, q[:, :0], w, w, pos, inv)
     assert torch.equal(without[0], with_keys[0]) and without[1].shape == (9, 0, 64) and not without[3].any()
+
+
+@pytest.mark.gpu
+def test_frequencies_that_would_lose_their_gradient_are_refused(pkg):
+    q, k, pos, inv = make(5, 4, 2, 64, 32, torch.bfloat16)
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    q.requires_grad_()
+    for learn in (False, True):
+        f = inv.clone().requires_grad_(learn)
+        for y, _ in (torch.ops.b200ht.rotary_qk(q, k, pos, f), torch.ops.b200ht.norm_rotary_qk(q, k, w, w, pos, f)):
+            if learn:
+                with pytest.raises(RuntimeError, match="inv_freq has no gradient"):
+                    y.float().sum().backward()
+            else:
+                q.grad = None
+                y.float().sum().backward()
+                assert q.grad.shape == q.shape
