@@ -669,3 +669,39 @@ def test_frequencies_that_would_lose_their_gradient_are_refused(pkg):
                 q.grad = None
                 y.float().sum().backward()
                 assert q.grad.shape == q.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,hq,hk,D,pairs,dtype", [
+    (4001, 8, 2, 128, 64, torch.bfloat16), (2500, 1, 64, 64, 32, torch.float16), (3000, 2, 1, 256, 128, torch.float32),
+    (5000, 3, 3, 80, 40, torch.bfloat16), (3001, 64, 1, 66, 33, torch.bfloat16), (2000, 1, 1, 80, 20, torch.float32),
+    (1, 1, 1, 128, 64, torch.bfloat16), (3, 0, 5, 96, 48, torch.float16),
+])
+def test_gradients_lie_between_untouched_zones(pkg, lib, T, hq, hk, D, pairs, dtype):
+    """The gradients inside larger rows, the weights' and the workspace of just the size asked for with a pattern on both
+    sides; enough tokens that the number of blocks, and so of the workspace's rows, reaches its limit."""
+    l = lib.load()
+    q, k, pos, inv = make(T, hq, hk, D, pairs, dtype, packed=True, far=99)
+    w = torch.linspace(0.5, 1.5, D, device="cuda").to(dtype)
+    gq, gk = torch.randn_like(q), torch.randn_like(k)
+    outs = [torch.full((T + 4, h + 1, D + 16), 7.0, dtype=dtype, device="cuda") for h in (hq, hk)]
+    dq, dk = outs[0][2:2 + T, :hq, 8:8 + D], outs[1][2:2 + T, :hk, 8:8 + D]
+    need, guard = l.b200ht_norm_rotary_qk_backward_workspace_bytes(D), 4096
+    ws = torch.full((need + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda")
+    dw = torch.full((3, 2, D), 7.0, dtype=dtype, device="cuda")
+    strides = (ctypes.c_longlong * 12)(*(s for x in (gq, gk, q, k, dq, dk) for s in x.stride()[:2]))
+    rc = l.b200ht_norm_rotary_qk_backward(
+        gq.data_ptr(), gk.data_ptr(), q.data_ptr(), k.data_ptr(), w.data_ptr(), w.data_ptr(), 1e-6, dq.data_ptr(), dk.data_ptr(),
+        dw[1, 0].data_ptr(), dw[1, 1].data_ptr(), T, hq, hk, D, strides, {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}[dtype],
+        pos.data_ptr(), 0, 1, 1, None, inv.data_ptr(), pairs, lib.ROT_POS64, ws.data_ptr() + guard, need,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.error_string(rc)
+    want = pkg.norm_rotary_qk_backward(gq, gk, q, k, w, w, pos, inv)
+    for a, b in zip((dq, dk, dw[1, 0], dw[1, 1]), want):
+        assert torch.equal(a, b)
+    for z in (ws[:guard], ws[guard + need:]):
+        assert bool((z == 0xA5).all())
+    assert bool((dw[0] == 7.0).all() and (dw[2] == 7.0).all())
+    for o, view in zip(outs, (dq, dk)):
+        view.fill_(7.0)
+        assert bool((o == 7.0).all())

@@ -496,7 +496,7 @@ BROKEN = [
     # tiles behind 256-row ones, tokens in chunks; the three ways a tile's results leave
     (40, 256, 140, 16, 6, "nm", torch.float32), (40, 256, 130, 16, 6, "mn", torch.bfloat16), (300, 512, 257, 128, 5, "nm", torch.bfloat16),
     (1500, 256, 4096, 72, 7, "mn", torch.float32), (1504, 256, 4096, 24, 7, "mn", torch.bfloat16), (1500, 256, 4096, 8, 7, "nm", torch.bfloat16),
-    (3000, 64, 4096, 16, 5, "nm", torch.bfloat16), (3000, 64, 4100, 16, 5, "mn", torch.float32), (1600, 16384, 64, 16, 4, "nm", torch.float32),
+    (2560, 64, 4096, 16, 5, "nm", torch.bfloat16), (2500, 64, 4090, 16, 5, "mn", torch.bfloat16), (3000, 64, 4100, 16, 5, "mn", torch.float32), (1600, 16384, 64, 16, 4, "nm", torch.float32),
 ]
 
 
@@ -570,3 +570,43 @@ def test_a_backward_that_saved_an_output_fails_once_it_is_overwritten(pkg):
         assert call(out) is out and torch.equal(out, call(torch.empty(shape, device="cuda")))
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entry,columns,K,M,R,L", [
+    # the streaming form: clusters of the front kernel, one column, tails of rows, few rows; then more columns than one pass
+    ("gemv", 16, 4096, 97, 16, 5), ("gemv", 8, 8192, 333, 128, 3), ("gemv", 1, 256, 1, 8, 1), ("gemv", 31, 1024, 4100, 72, 4),
+    ("gemv", 2, 512, 7, 24, 2), ("gemv", 20, 8192, 50, 16, 4), ("gemv", 64, 4096, 40, 16, 4), ("gemv", 5, 32768, 9, 40, 2),
+    ("mn", 16, 4096, 97, 16, 5), ("nm", 16, 4096, 97, 16, 5), ("mn", 3, 8192, 130, 120, 2), ("nm", 1, 256, 2000, 8, 3),
+    ("nm", 64, 4096, 130, 32, 6), ("mn", 2600, 64, 4090, 8, 40),
+])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_c_entries_write_between_their_guards(pkg, lib, entry, columns, K, M, R, L, dtype):
+    """Workspaces and results of just the size asked for, with a pattern on both sides."""
+    l = lib.load()
+    X, W, A, B, index, scaling = make(columns, K, M, R, L, seed=23, spread="any")
+    Xc = X.t().contiguous()
+    odt, guard = (lib.F32 if dtype == torch.float32 else lib.BF16), 4096
+    nc = M * columns * (4 if dtype == torch.float32 else 2)
+    n = l.b200ht_lora_gemv_workspace_bytes(M, K, columns, R) if entry == "gemv" else l.b200ht_lora_gemm_workspace_bytes(M, columns, K, R)
+    ws, C = (torch.full((size + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda") for size in (n, nc))
+    at = ws.data_ptr() + guard
+    assert at % 256 == 0
+    stream = torch.cuda.current_stream().cuda_stream
+    if entry == "gemv":
+        rc = l.b200ht_lora_gemv(W.data_ptr(), Xc.data_ptr(), C.data_ptr() + guard, A.data_ptr(), B.data_ptr(), index.data_ptr(),
+                                scaling.data_ptr(), M, K, columns, L, R, odt, K ** -0.5, at, n, stream)
+    else:
+        rc = l.b200ht_lora_gemm(X.data_ptr(), W.data_ptr(), C.data_ptr() + guard, A.data_ptr(), B.data_ptr(), index.data_ptr(),
+                                scaling.data_ptr(), M, columns, K, L, R, odt, lib.OUT_NM if entry == "nm" else lib.OUT_MN, K ** -0.5,
+                                None, at, n, stream)
+    assert rc == 0, lib.error_string(rc)
+    for z in (ws[:guard], ws[guard + n:], C[:guard], C[guard + nc:]):
+        assert bool((z == 0xA5).all())
+    got = C[guard:guard + nc].view(dtype).view((columns, M) if entry == "nm" else (M, columns))
+    want = share64(X, A, B, index, scaling)[0]
+    got = (got if entry == "nm" else got.t()).double().cpu()
+    # that something was written: far closer to the definition than the results are large (their bounds are tested above)
+    base = pkg.lora_ht_gemm(X, W, A, B, torch.full_like(index, -1), out_layout="nm").double().cpu()
+    assert float((got - want - base).norm() / (want + base).norm()) <= 2.0 ** -5
+    assert pkg.device_status() == 0
