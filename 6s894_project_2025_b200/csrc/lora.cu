@@ -409,10 +409,9 @@ lora_expand_kernel(const float *base, const __nv_bfloat16 *B, const float *S, co
 // S of many tokens, on the tensor cores: 256 tokens (the N of the instruction) against the A matrices of the adapters among
 // them, 128 / rank of which share the M of one instruction, two such groups a pass; K is split over the CTAs of a cluster.
 // Each token keeps the rows of its own adapter.  With prompts a tile has a few adapters, one pass serves them and X is read
-// once; bound then: the bytes of X.  (An instruction takes about 90 ns whatever its M and N, so it should be full: with 128
-// tokens as M and an instruction an adapter, 16384 x 8192 tokens of 40 requests at rank 64 took 94 us; with the adapters as
-// M and 128 tokens as N, 97 us, two tiles an SM taking turns and a second pass where a tile had three adapters; so 71 us,
-// 41 at the copy bandwidth.)  Short prompts are bound by the chain of latencies: 2001 x 4096 at rank 32 takes 14 us.
+// once; bound then: the bytes of X.  (Full instructions pay: with 128 tokens as M and an instruction an adapter, 16384 x
+// 8192 tokens of 40 requests at rank 64 took 94 us; with the adapters as M and 128 tokens as N, 97 us, two tiles an SM
+// taking turns and a second pass where a tile had three adapters; so 71 us, 41 at the copy bandwidth.)  Short prompts are bound by the chain of latencies: 2001 x 4096 at rank 32 takes 14 us.
 //
 // Warp 0 copies by TMA (X 256 x 64 and rank x 64 of each adapter's A a stage, 128-byte swizzle), warp 1 issues the MMAs,
 // warps 2..9 find the tile's adapters while the first tiles of X arrive, and at the end bring the accumulators (one row of
@@ -656,8 +655,12 @@ int launch_lora_transform(const void *X, void *Y, int tokens, int K, float scale
 }
 
 // Few tokens: blocks for each, which read its A through L2 (3 TB/s or so, whatever the tokens' order); from 32 MB of such
-// reads on the tile kernel, whose time goes by the adapters of a tile.  At 256 tokens, K = 4096, rank 16 (32 MB): 12 us
-// against 13 (one adapter) and 29 (64 adapters).
+// reads on the tile kernel, whose time goes by the adapters of a tile.  Whole calls at M = 1024, rows / tiles, us: K = 4096,
+// rank 16, 128 tokens (16 MB) of one adapter 22.0 / 21.5, of eight 22.0 / 23.7; 256 tokens (32 MB) 26.3 / 25.6, 26.8 / 27.8;
+// 512 (64 MB) 42 / 37, 43 / 38; 1024 (128 MB) 42 / 29, 42 / 30; rank 64, 64 tokens (32 MB) 22.5 / 20.9, 22.7 / 24.9; K = 1024,
+// rank 64, 256 tokens (32 MB) 23.2 / 22.9, 23.3 / 24.7, 1024 (128 MB) 43 / 24; K = 8192, rank 16, 128 tokens (32 MB) 26.5 /
+// 26.4, 26.5 / 31.4.  With 64 adapters in mixed order the rows stay ahead by a quarter beyond (1024 tokens 63 / 75), which
+// the host cannot see.
 static bool shrink_by_rows(int tokens, int K, int rank) { return (size_t)tokens * rank * K * 2 <= (size_t)32 << 20; }
 
 static int launch_shrink_tiles(const void *X, const void *A, const int *index, const float *scaling, __nv_bfloat16 *S, int tokens, int K,
@@ -760,7 +763,9 @@ extern "C" int b200ht_lora_gemm(const void *X, const void *W, void *C, const voi
     rc = check_device();
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    // as few tokens as the streaming GEMV serves with one pass over W: 17 us for 16 of them at 4096 x 4096, 24 by what follows
+    // as few tokens as the streaming GEMV serves with one pass over W; us, so / by what follows: 16 tokens at 4096 x 4096
+    // 15 / 23, 4096 x 28672 72 / 101; 8 at 8192 x 1024 14.0 / 15.7, 8192 x 28672 105 / 124; 24 at 2048 x 4096 12.6 / 17.6; 32 at
+    // 1024 x 4096 16.1 / 16.0, 512 x 512 13.7 / 14.7; one token 7.5 / 11.7 to 77 / 198
     if (!signs && gemv_adapt_shape(K, N)) {
         const bool mn = out_layout == B200HT_OUT_MN;
         return lora_stream(W, X, true, C, mn ? (size_t)N : 1, mn ? 1 : (size_t)M, A, B, index, scaling, M, K, N, adapters, rank, out_dtype,

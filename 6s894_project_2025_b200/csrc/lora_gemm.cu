@@ -8,9 +8,9 @@
 //               after all earlier work (lora_plan_kernel), so W is complete.
 //   warp 1      tcgen05.mma (M = 128, N = box, K = 16); masks S as gemm_tcgen05.cu does
 //   warps 2..5  the accumulator into shared memory, over the used stages, one row of W a lane
-// Bound: the bytes of W; per CTA the issue of the MMAs (an instruction costs the same whatever its N, so K is what is
-// split).  64 tokens of 16 adapters (rank 16) at 4096 x 4096: 25 us with everything in front, 50 by the tiles of
-// gemm_tcgen05.cu.  Every wait is time-limited; a CTA whose wait ran out keeps step with its cluster and leaves
+// Bound: the bytes of W, and the chain of four launches (plan, S, H(X), this), each of which waits for its latencies; a
+// CTA's time goes by its K steps, hence the split over K.  64 tokens of 16 adapters (rank 16) at 4096 x 4096: 24 us with
+// everything in front (6 at the copy bandwidth), 50 by the tiles of gemm_tcgen05.cu.  Every wait is time-limited; a CTA whose wait ran out keeps step with its cluster and leaves
 // B200HT_ERR_TIMEOUT in the status word.
 #include "lora_tc.cuh"
 

@@ -84,9 +84,11 @@ __device__ __forceinline__ float warp_sum(float v)
 }
 
 // ---------------------------------------------------------------------------
-// Any head dimension, stride and alignment: a warp per row, the row in shared memory as fp32, one element per lane and
-// step.  About ten times slower than the fast form below (32768 x 40 x 128 with H: 1460 us against 138), for rows that it
-// does not take.
+// Any head dimension, stride, alignment and number of pairs: a warp per row, the row in shared memory as fp32, one element
+// per lane and step.  Six to eleven times the floor (the fast form below 1.1 to 1.7), for rows that it does not take: heads
+// that are no multiple of 16 (72: 311 us for 16384 x 40, floor 29), rows off a 16-byte boundary, and split pairs of which
+// some dimensions stay where they are, unless they are a multiple of 8 in the first half of the head (128 with 96 turning:
+// 320 us, with neighbouring pairs 58, floor 51; 80 with 40 turning: 201 us, floor 32).
 // ---------------------------------------------------------------------------
 constexpr int kAnyWarps = 4;
 
@@ -221,8 +223,9 @@ norm_rotary_any_grad_kernel(const __grid_constant__ RotArgs a, int q_blocks)
 // their pairs are computed once into shared memory and serve all heads, each group walks over heads of one token with
 // the next row's loads in flight.  Bound: HBM without H, the instruction rate with it (160 issued instructions per 512
 // values and warp, 330 with H), hence the packed fp32 instructions: 66 us against 73 without them.
-// 16384 tokens x 40 heads x 128, bf16 (51 us at the copy bandwidth): rotation 62 us, with H 66, norm 65, norm with H 76; four
-// resident blocks an SM (64 registers) measured best, three 65 / 70 / 68 / 77, five spill (68 / 104 / 92 / 122).
+// 16384 tokens x 40 heads x 128, bf16 (51 us at the copy bandwidth): rotation 59 us, with H 63, norm 64, norm with H 77; four
+// resident blocks an SM (64 registers) measured best (62 / 66 / 65 / 76 then), three 65 / 70 / 68 / 77, five spill (68 / 104
+// / 92 / 122).  fp32, 8192 x 18 x 256 (46 us): rotation 60 us, norm 63; a lane's 32 bytes leave as two halves of a sector.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
@@ -578,7 +581,7 @@ rotary_row_kernel(const __grid_constant__ RotArgs a, int tb, int mode)
 // table of cos and sin the blocks stood still for a fifth of the time.  Registers are what limits it: the next row comes
 // by cp.async into a slot of shared memory that its own thread (fp32: group) alone reads, x is read from there once for
 // each of its three uses, and for split pairs cos and sin stay in shared memory as well.  16384 tokens x 40 heads x 128,
-// bf16: 90 us, 77 at the copy bandwidth; 127 with H (instruction rate).
+// bf16: 90 - 95 us, 77 at the copy bandwidth; 127 with H (instruction rate).
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void *src)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
@@ -856,7 +859,7 @@ static GradBlocks grad_blocks(double q_work, double k_work, double work_per_bloc
     return b;
 }
 // Blocks of a gradient launch at most (one more may come from rounding up).  They do not go by the device's number of
-// SMs, so that the order of the sums goes by the sizes alone.
+// SMs, so that the order of the sums is the same on each.
 constexpr int kGradBlocks = 148 * 8;
 constexpr int row_grad_blocks(int dtype) { return 148 * (dtype == B200HT_F32 ? 2 : 3); }   // one wave of resident blocks
 

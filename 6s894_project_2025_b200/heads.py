@@ -226,7 +226,7 @@ def norm_rotary_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
 
     ``dq_out`` and ``dk_out`` are the gradients of its results, the other arguments those of the call (``q`` and ``k``
     before it: a call in place has lost them).  Without keys pass tensors of none, ``q[:, :0]``.  The weights' gradients are sums over all tokens and heads, in fp32 and
-    in an order that depends on the sizes alone.
+    in an order that depends on the sizes, the type and the layout (strides, alignment, order of the pairs) alone.
     """
     D, tokens, pairs, flags, table, n_axes, pa, pt = _check_common(q, positions, inv_freq, sections, axis_order, hadamard)
     if k is None or dk_out is None:
