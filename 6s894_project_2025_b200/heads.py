@@ -6,7 +6,8 @@ has no counterpart: its users would run the position rotation elsewhere and csrc
 (csrc/hadamard_transform.cpp:12-70).
 
 Tensors are (tokens, heads, head_dim); views of one packed projection are taken as they are.  All arithmetic happens in
-libb200ht.so (fp32, angles reduced in fp64, one rounding on the store); there is no CPU path.
+libb200ht.so (fp32, angles reduced in fp64, one rounding on the store); there is no CPU path.  These
+functions record no graph; ``torch.ops.b200ht.rotary_qk`` and ``norm_rotary_qk`` are the forms that differentiate.
 """
 from __future__ import annotations
 
